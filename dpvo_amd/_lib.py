@@ -13,8 +13,8 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DPVO_HIP_LIB") or os.path.join(_HERE, "libdpvo_hip.so")      # (override: development builds)
 
-F16, F32 = 0, 1
-ABI_VERSION = 8         # == DPVO_ABI_VERSION of include/dpvo_hip.h this binding (struct layouts, signatures) was written against
+F16, F32, BF16 = 0, 1, 2
+ABI_VERSION = 9         # == DPVO_ABI_VERSION of include/dpvo_hip.h this binding (struct layouts, signatures) was written against
 
 # every symbol include/dpvo_hip.h declares (tests/test_capi.py checks the .so exports all of them)
 SYMBOLS = [
@@ -34,6 +34,9 @@ SYMBOLS = [
     "dpvo_normalize_image", "dpvo_patch_colors", "dpvo_store_features", "dpvo_append_edges", "dpvo_gather_edges", "dpvo_gather_edges2",
     "dpvo_motion_model", "dpvo_median_depth", "dpvo_frame_patches", "dpvo_frame_state", "dpvo_frame_state_part", "dpvo_keyframe_step", "dpvo_frame_update", "dpvo_debug_stamp",
     "dpvo_encoders_workspace_bytes", "dpvo_encoders_forward", "dpvo_encoders_forward_hold", "dpvo_pool4_nhwc",
+    "dpvo_gated_linear", "dpvo_gated_linear_dact", "dpvo_gated_linear_dx_workspace_bytes", "dpvo_gated_linear_dx",
+    "dpvo_gated_linear_dw_workspace_bytes", "dpvo_gated_linear_dw",
+    "dpvo_residual_norm", "dpvo_residual_norm_backward_workspace_bytes", "dpvo_residual_norm_backward",
 ]
 
 
@@ -101,6 +104,38 @@ class PlanLayout(ctypes.Structure):
                  "total_ints", "flow")]
 
 
+class GatedLinear(ctypes.Structure):
+    """dpvo_gated_linear_t"""
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("x", "v", "w_gate", "w_up", "b_gate", "b_up", "residual", "y", "save_gate", "save_up")] +
+                [(k, ctypes.c_int64) for k in ("ldx", "ldv", "ldwg", "ldwu", "ldr", "ldy", "M", "N", "K", "Kv")] +
+                [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32)])
+
+
+class GatedLinearDx(ctypes.Structure):
+    """dpvo_gated_linear_dx_t"""
+    _fields_ = ([("a", ctypes.c_void_p * 2), ("b", ctypes.c_void_p * 2)] +
+                [(k, ctypes.c_void_p) for k in ("addend", "mask", "gate", "up", "dx", "dx2")] +
+                [(k, ctypes.c_int64 * 2) for k in ("lda", "ldb", "K")] +
+                [(k, ctypes.c_int64) for k in ("ldadd", "ldmask", "lddx", "M", "N")] +
+                [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32)])
+
+
+class GatedLinearDw(ctypes.Structure):
+    """dpvo_gated_linear_dw_t"""
+    _fields_ = ([(k, ctypes.c_void_p * 4) for k in ("a", "b", "dw", "db")] +
+                [(k, ctypes.c_int64 * 4) for k in ("lda", "ldb", "N", "K")] +
+                [("M", ctypes.c_int64), ("n", ctypes.c_int32), ("dtype", ctypes.c_int32)])
+
+
+class ResidualNorm(ctypes.Structure):
+    """dpvo_residual_norm_t"""
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("x", "f", "gate", "w", "b", "pw", "pb", "s", "h", "ds", "dh", "dx", "df", "dgate", "dw",
+                                                "db", "dpw", "dpb")] +
+                [(k, ctypes.c_int64) for k in ("ldx", "ldf", "ldgate", "ldds", "lddh", "M", "groups")] +
+                [(k, ctypes.c_int32) for k in ("D", "x_dtype", "f_dtype", "h_dtype", "w_dtype", "norm", "post", "gate_activation")] +
+                [(k, ctypes.c_float) for k in ("scale", "eps", "post_eps")])
+
+
 _lib = None
 
 
@@ -117,8 +152,16 @@ def lib():
                 raise DPVOHipError(f"libdpvo_hip.so does not export {s}")
         for s in ("dpvo_plan_workspace_bytes", "dpvo_plan_wide_workspace_bytes", "dpvo_normalize_scratch_bytes", "dpvo_neighbors_workspace_bytes", "dpvo_ba_workspace_bytes",
                   "dpvo_gba_workspace_bytes", "dpvo_gba_solve_workspace_bytes", "dpvo_solve_system_workspace_bytes", "dpvo_encoders_workspace_bytes",
-                  "dpvo_update_fused_workspace_bytes", "dpvo_update_fused_pack_bytes"):
+                  "dpvo_update_fused_workspace_bytes", "dpvo_update_fused_pack_bytes", "dpvo_gated_linear_dx_workspace_bytes",
+                  "dpvo_gated_linear_dw_workspace_bytes", "dpvo_residual_norm_backward_workspace_bytes"):
             getattr(L, s).restype = ctypes.c_size_t
+        vp, i64_, i32_ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+        L.dpvo_gated_linear.argtypes = [vp, vp]
+        L.dpvo_gated_linear_dact.argtypes = [vp, i64_, vp, vp, vp, vp, i64_, i32_, i32_, i64_, i64_, vp]
+        L.dpvo_gated_linear_dx_workspace_bytes.argtypes = [i64_, i64_, i64_]
+        L.dpvo_gated_linear_dw_workspace_bytes.argtypes = L.dpvo_residual_norm_backward_workspace_bytes.argtypes = [vp]
+        L.dpvo_gated_linear_dx.argtypes = L.dpvo_gated_linear_dw.argtypes = L.dpvo_residual_norm_backward.argtypes = [vp, vp, ctypes.c_size_t, vp]
+        L.dpvo_residual_norm.argtypes = [vp, vp]
         L.dpvo_abi_version.restype = ctypes.c_int
         if L.dpvo_abi_version() != ABI_VERSION:
             raise DPVOHipError(f"{LIB_PATH} has ABI version {L.dpvo_abi_version()}, this binding needs {ABI_VERSION}: rebuild it "

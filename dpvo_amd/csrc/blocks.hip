@@ -1,0 +1,434 @@
+// blocks.hip -- C entries of the gated feed-forward blocks and the norms around them (include/dpvo_hip.h), their small kernels, and the
+// choice of tiles and splits.  The products themselves: blocks_gemm.h; the norms: blocks_norm.h.
+#include <limits.h>
+#include "blocks_dev.h"
+#include "blocks_norm.h"
+
+namespace blk {
+namespace {
+
+inline bool type_ok(int t) { return t == DPVO_F16 || t == DPVO_BF16 || t == DPVO_F32; }
+inline int type_size(int t) { return t == DPVO_F32 ? 4 : 2; }
+inline bool act_ok(int a) { return a >= DPVO_ACT_IDENTITY && a <= DPVO_ACT_GELU_TANH; }
+// row offsets within a tile are 32-bit bytes
+inline bool ld_ok(int64_t ld, int64_t width, int size) { return ld >= width && ld <= INT_MAX / (256 * size); }
+
+int gemm(const GemmArgs& a, int dtype, int form, int epi, int big, int64_t tiles, hipStream_t s) {
+  if (tiles > INT_MAX) return DPVO_E_UNSUPPORTED;
+  if (dtype == DPVO_F16) return gemm_f16(a, form, epi, big, tiles, s);
+  if (dtype == DPVO_BF16) return gemm_bf16(a, form, epi, big, tiles, s);
+  return gemm_f32(a, form, epi, big, tiles, s);
+}
+inline int block_k(int dtype) { return dtype == DPVO_F32 ? 32 : 64; }
+
+// Parts a sum over `nb` blocks is cut into when its `tiles` tiles are too few for the chip: two workgroups on each of 256 compute units, but at
+// least 8 blocks to a part (a part costs a tile's write and read in f32).
+int64_t splits_for(int64_t tiles, int64_t nb) {
+  if (tiles <= 0) return 1;
+  int64_t s = 512 / tiles;
+  if (s > nb / 8) s = nb / 8;
+  return s < 1 ? 1 : s > 64 ? 64 : s;
+}
+
+// out[e] = sum over splits of part[split][e] (+ addend[e]), all contiguous
+template <class T> __global__ void __launch_bounds__(256) split_sum_kernel(const float* part, int64_t size, int splits, const T* addend, T* out) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= size) return;
+  const int nv = size - e < 4 ? (int)(size - e) : 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, t[4];
+  for (int s = 0; s < splits; ++s) {
+    load_n<float, 4>(part + s * size + e, nv, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += t[i];
+  }
+  if (addend) {
+    load_n<T, 4>(addend + e, nv, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += t[i];
+  }
+  store_n<T, 4>(out + e, nv, v);
+}
+int split_sum(const float* part, int64_t size, int splits, const void* addend, void* out, int dtype, hipStream_t s) {
+  if (size == 0) return DPVO_OK;
+  const int64_t blocks = cdiv64(cdiv64(size, 4), 256);
+  if (blocks > INT_MAX) return DPVO_E_UNSUPPORTED;
+  if (dtype == DPVO_F16) hipLaunchKernelGGL((split_sum_kernel<_Float16>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const _Float16*)addend, (_Float16*)out);
+  else if (dtype == DPVO_BF16) hipLaunchKernelGGL((split_sum_kernel<__bf16>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const __bf16*)addend, (__bf16*)out);
+  else hipLaunchKernelGGL((split_sum_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const float*)addend, (float*)out);
+  DPVO_LAUNCH_CHECK();
+  return DPVO_OK;
+}
+
+// dpvo_gated_linear_dact: one pass, 8 elements a thread
+template <class T> __global__ void __launch_bounds__(256) dact_kernel(const T* dy, int64_t lddy, const float* gate, const float* up, T* dg, T* du, int64_t ldo,
+                                                                       int act, int64_t M, int64_t N) {
+  const int64_t n8 = (N + 7) / 8, total = M * n8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / n8, n = (i % n8) * 8;
+    const int nv = N - n < 8 ? (int)(N - n) : 8;
+    float d[8], g[8], u[8];
+    load_n<T, 8>(dy + m * lddy + n, nv, d);
+    load_n<float, 8>(gate + m * N + n, nv, g);
+    if (up) load_n<float, 8>(up + m * N + n, nv, u);
+    float o[8];
+    act_d8<sizeof(T) == 4>(act, g, o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[e] *= d[e];
+      d[e] *= up ? u[e] * g[e] : g[e];
+    }
+    store_n<T, 8>(dg + m * ldo + n, nv, d);
+    if (up) store_n<T, 8>(du + m * ldo + n, nv, o);
+  }
+}
+
+// ---- column sums: rows -> partial rows (a workgroup: 256 columns, its share of the rows), partial rows -> one
+struct ColJob {
+  const void* a;
+  float* part;
+  void* out;
+  int64_t lda, M, N;                                     // M rows of N
+  int64_t parts;                                         // partial rows to one output row
+  int64_t outs;                                          // output rows
+  int type;                                              // of `a` (first pass), of `out` (second)
+};
+struct ColArgs {
+  ColJob j[5];
+  int n;
+};
+template <class T> __device__ __forceinline__ void col_rows(const T* a, int64_t lda, int64_t r0, int64_t r1, int nv, float (&v)[8]) {
+  float t[8];
+  for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += 8) {
+    load_n<T, 8>(a + r * lda, nv, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+}
+__global__ void __launch_bounds__(256) col_sum_kernel(const ColArgs args) {
+  __shared__ float lds[8][256 + 8];
+  const ColJob& j = args.j[blockIdx.z];
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x % 32 * 8;
+  if ((int64_t)blockIdx.x * 256 >= j.N) return;          // (another job's columns; the whole workgroup)
+  const int64_t r0 = j.M * blockIdx.y / gridDim.y, r1 = j.M * (blockIdx.y + 1) / gridDim.y;
+  float v[8] = {};
+  if (n < j.N) {
+    const int nv = j.N - n < 8 ? (int)(j.N - n) : 8;
+    if (j.type == DPVO_F16) col_rows((const _Float16*)j.a + n, j.lda, r0, r1, nv, v);
+    else if (j.type == DPVO_BF16) col_rows((const __bf16*)j.a + n, j.lda, r0, r1, nv, v);
+    else col_rows((const float*)j.a + n, j.lda, r0, r1, nv, v);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) lds[threadIdx.x / 32][threadIdx.x % 32 * 8 + e] = v[e];
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c < j.N) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += lds[k][threadIdx.x];
+    j.part[blockIdx.y * j.N + c] = s;
+  }
+}
+// out[o][c] = sum of part[o * parts + p][c]: 64 columns x 4 shares of the partial rows
+__global__ void __launch_bounds__(256) col_reduce_kernel(const ColArgs args) {
+  __shared__ float lds[4][64];
+  const ColJob& j = args.j[blockIdx.z];
+  const int64_t c0 = (int64_t)blockIdx.x * 64, c = c0 + threadIdx.x % 64;
+  if (c0 >= j.N) return;
+  for (int64_t o = blockIdx.y; o < j.outs; o += gridDim.y) {
+    float s = 0.f;
+    if (c < j.N)
+      for (int64_t p = threadIdx.x / 64; p < j.parts; p += 4) s += j.part[(o * j.parts + p) * j.N + c];
+    lds[threadIdx.x / 64][threadIdx.x % 64] = s;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < j.N) {
+      s = ((lds[0][threadIdx.x] + lds[1][threadIdx.x]) + lds[2][threadIdx.x]) + lds[3][threadIdx.x];
+      if (j.type == DPVO_F16) ((_Float16*)j.out)[o * j.N + c] = (_Float16)s;
+      else if (j.type == DPVO_BF16) ((__bf16*)j.out)[o * j.N + c] = (__bf16)s;
+      else ((float*)j.out)[o * j.N + c] = s;
+    }
+    __syncthreads();
+  }
+}
+int col_reduce(const ColArgs& c, hipStream_t s) {
+  if (c.n == 0) return DPVO_OK;
+  int64_t w = 0, o = 0;
+  for (int i = 0; i < c.n; ++i) {
+    w = c.j[i].N > w ? c.j[i].N : w;
+    o = c.j[i].outs > o ? c.j[i].outs : o;
+  }
+  if (w == 0 || o == 0) return DPVO_OK;
+  hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)cdiv64(w, 64), (unsigned)(o < 1024 ? o : 1024), (unsigned)c.n), dim3(256), 0, s, c);
+  DPVO_LAUNCH_CHECK();
+  return DPVO_OK;
+}
+int64_t col_parts(int64_t M) { return M < 64 ? 1 : M / 64 < 256 ? M / 64 : 256; }
+
+void tiles_of(Prob& p, int tm, int tn) {
+  p.tm = cdiv64(p.M, tm);
+  p.tn = cdiv64(p.N, tn);
+}
+
+// ---- the norm backward's share of rows
+struct NormPlan {
+  NormShape sh;
+  int64_t groups, rpg, gpb, bpg, blocks;
+  bool shared;                                           // the gate's gradient is summed over rows
+};
+NormPlan norm_plan(const dpvo_residual_norm_t& p) {
+  NormPlan n;
+  n.sh = norm_shape(p.D);
+  n.shared = p.f && p.gate && p.dgate && p.groups < p.M;
+  n.groups = n.shared ? p.groups : 1;
+  n.rpg = n.groups ? p.M / n.groups : 0;
+  // 512 workgroups: enough loads in flight for the memory, few enough that their partial rows stay a few per cent of the traffic
+  const int64_t want = 512, rounds = cdiv64(n.rpg, norm_slots(n.sh));
+  if (n.groups >= want) {
+    n.bpg = 1;
+    n.gpb = cdiv64(n.groups, want);
+  } else {
+    n.gpb = 1;
+    n.bpg = want / n.groups;
+    if (n.bpg > rounds) n.bpg = rounds < 1 ? 1 : rounds;
+  }
+  n.blocks = cdiv64(n.groups, n.gpb) * n.bpg;
+  return n;
+}
+int norm_check(const dpvo_residual_norm_t* p) {
+  if (!p || p->M < 0 || p->D < 1 || !type_ok(p->x_dtype) || !type_ok(p->f_dtype) || !type_ok(p->w_dtype)) return DPVO_E_INVALID;
+  if (p->x_dtype != p->f_dtype && p->x_dtype != DPVO_F32) return DPVO_E_UNSUPPORTED;
+  if (p->h_dtype != p->x_dtype && p->h_dtype != p->f_dtype) return DPVO_E_UNSUPPORTED;
+  if (p->norm < DPVO_NORM_NONE || p->norm > DPVO_NORM_RMS || p->post < DPVO_NORM_NONE || p->post > DPVO_NORM_RMS) return DPVO_E_INVALID;
+  if (!act_ok(p->gate_activation)) return DPVO_E_INVALID;
+  if (p->D > NORM_MAX_D) return DPVO_E_UNSUPPORTED;
+  if (p->gate && (p->groups < 1 || p->M % p->groups || !p->f)) return DPVO_E_INVALID;
+  if (p->M && !p->x) return DPVO_E_INVALID;
+  return DPVO_OK;
+}
+int norm_run(const NormArgs& a, const NormShape& sh, bool back, int64_t blocks, hipStream_t s) {
+  if (a.p.f_dtype == DPVO_F16) return norm_f16(a, sh, back, blocks, s);
+  if (a.p.f_dtype == DPVO_BF16) return norm_bf16(a, sh, back, blocks, s);
+  return norm_f32(a, sh, back, blocks, s);
+}
+
+}  // namespace
+}  // namespace blk
+
+using namespace blk;
+
+extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream) {
+  if (!p || !type_ok(p->dtype) || !act_ok(p->activation) || p->M < 0 || p->N < 0 || p->K < 0 || p->Kv < 0) return DPVO_E_INVALID;
+  if (p->M == 0 || p->N == 0) return DPVO_OK;
+  const int size = type_size(p->dtype);
+  if (!p->y || (p->K && (!p->x || !p->w_gate)) || (p->w_up && p->Kv && !p->v)) return DPVO_E_INVALID;
+  if (!ld_ok(p->ldx, p->K, size) || !ld_ok(p->ldwg, p->K, size) || p->ldy < p->N || (p->residual && p->ldr < p->N)) return DPVO_E_INVALID;
+  if (p->w_up && (!ld_ok(p->ldv, p->Kv, size) || !ld_ok(p->ldwu, p->Kv, size))) return DPVO_E_INVALID;
+  const bool same = p->w_up && p->v == p->x && p->ldv == p->ldx && p->Kv == p->K;
+  GemmArgs a = {};
+  a.n = 1;
+  Prob& q = a.p[0];
+  q.A[0] = p->x; q.B[0] = p->w_gate; q.lda[0] = p->ldx; q.ldb[0] = p->ldwg; q.K[0] = p->K;
+  q.A[1] = p->v; q.B[1] = p->w_up; q.lda[1] = p->ldv; q.ldb[1] = p->ldwu; q.K[1] = p->Kv;
+  q.M = p->M; q.N = p->N;
+  q.bias0 = p->b_gate; q.bias1 = p->b_up; q.addend = p->residual; q.ldadd = p->ldr;
+  q.out0 = p->y; q.ldo = p->ldy; q.save0 = p->save_gate; q.save1 = p->w_up ? p->save_up : nullptr;
+  q.act = p->activation; q.splits = 1;
+  const int bk = block_k(p->dtype), epi = !p->w_up ? E_LIN : same ? E_GATE : E_GATE2;
+  q.nb0 = cdiv64(p->K, bk);
+  q.nb = q.nb0 + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0);
+  tiles_of(q, 128, epi == E_GATE ? 64 : 128);
+  return gemm(a, p->dtype, F_NT, epi, 0, q.tm * q.tn, (hipStream_t)stream);
+}
+
+extern "C" int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, const float* up, void* d_gate, void* d_up, int64_t ldo, int dtype,
+                                      int activation, int64_t M, int64_t N, void* stream) {
+  if (!type_ok(dtype) || !act_ok(activation) || M < 0 || N < 0) return DPVO_E_INVALID;
+  if (M == 0 || N == 0) return DPVO_OK;
+  if (!dy || !gate || !d_gate || (up && !d_up) || lddy < N || ldo < N) return DPVO_E_INVALID;
+  const int64_t want = cdiv64(M * cdiv64(N, 8), 256), blocks = want < 16384 ? want : 16384;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DPVO_F16) hipLaunchKernelGGL((dact_kernel<_Float16>), dim3((unsigned)blocks), dim3(256), 0, s, (const _Float16*)dy, lddy, gate, up, (_Float16*)d_gate, (_Float16*)d_up, ldo, activation, M, N);
+  else if (dtype == DPVO_BF16) hipLaunchKernelGGL((dact_kernel<__bf16>), dim3((unsigned)blocks), dim3(256), 0, s, (const __bf16*)dy, lddy, gate, up, (__bf16*)d_gate, (__bf16*)d_up, ldo, activation, M, N);
+  else hipLaunchKernelGGL((dact_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)dy, lddy, gate, up, (float*)d_gate, (float*)d_up, ldo, activation, M, N);
+  DPVO_LAUNCH_CHECK();
+  return DPVO_OK;
+}
+
+// (the workspace does not know the type: blocks of 32 are the finer cut)
+static int64_t dx_splits(int64_t M, int64_t N, int64_t K, int bk) { return splits_for(cdiv64(M, 128) * cdiv64(N, 128), cdiv64(K, bk)); }
+
+extern "C" size_t dpvo_gated_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int64_t s = dx_splits(M, N, K + 64, 32);
+  return s > 1 ? (size_t)(s * M * N * 4) : 0;
+}
+
+extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, size_t ws_bytes, void* stream) {
+  if (!p || !type_ok(p->dtype) || !act_ok(p->activation) || p->M < 0 || p->N < 0 || p->K[0] < 0 || p->K[1] < 0) return DPVO_E_INVALID;
+  if (p->M == 0 || p->N == 0) return DPVO_OK;
+  const int size = type_size(p->dtype), bk = block_k(p->dtype);
+  if (!p->dx || p->lddx < p->N || (p->addend && p->ldadd < p->N) || (p->mask && p->ldmask < p->N)) return DPVO_E_INVALID;
+  if ((p->gate || p->mask) && p->addend) return DPVO_E_UNSUPPORTED;
+  if ((p->gate && p->mask) || (p->up && (!p->gate || !p->dx2))) return DPVO_E_INVALID;
+  const int64_t K1 = p->a[1] ? p->K[1] : 0;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t k = i ? K1 : p->K[0];
+    if (k && (!p->a[i] || !p->b[i])) return DPVO_E_INVALID;
+    if (k && (!ld_ok(p->lda[i], k, size) || !ld_ok(p->ldb[i], p->N, size))) return DPVO_E_INVALID;
+  }
+  GemmArgs a = {};
+  a.n = 1;
+  Prob& q = a.p[0];
+  for (int i = 0; i < 2; ++i) {
+    q.A[i] = p->a[i]; q.B[i] = p->b[i]; q.lda[i] = p->lda[i]; q.ldb[i] = p->ldb[i];
+  }
+  q.K[0] = p->K[0]; q.K[1] = K1;
+  q.M = p->M; q.N = p->N;
+  q.out0 = p->dx; q.out1 = p->dx2; q.ldo = p->lddx; q.act = p->activation;
+  q.nb0 = cdiv64(p->K[0], bk);
+  q.nb = q.nb0 + cdiv64(K1, bk);
+  q.splits = 1;
+  tiles_of(q, 128, 128);
+  hipStream_t s = (hipStream_t)stream;
+  if (p->gate || p->mask) {
+    q.save0 = (float*)p->gate; q.save1 = (float*)p->up; q.mask = p->mask; q.ldmask = p->ldmask;
+    return gemm(a, p->dtype, F_NN, E_DACT, 0, q.tm * q.tn, s);
+  }
+  q.act = DPVO_ACT_IDENTITY;
+  const bool flat = p->lddx == p->N && (!p->addend || p->ldadd == p->N);
+  const int64_t splits = flat ? splits_for(q.tm * q.tn, q.nb) : 1;
+  if (splits > 1) {
+    if ((size_t)(splits * p->M * p->N * 4) > ws_bytes || !ws) return DPVO_E_WORKSPACE;
+    q.splits = (int)splits;
+    q.part = (float*)ws;
+    const int rc = gemm(a, p->dtype, F_NN, E_LIN, 0, q.tm * q.tn * splits, s);
+    return rc ? rc : split_sum(q.part, p->M * p->N, q.splits, p->addend, p->dx, p->dtype, s);
+  }
+  q.addend = p->addend; q.ldadd = p->ldadd;
+  return gemm(a, p->dtype, F_NN, E_LIN, 0, q.tm * q.tn, s);
+}
+
+// workspace: the parts of each product that is split, then the partial column sums
+static int64_t dw_splits(const dpvo_gated_linear_dw_t* p) {
+  int64_t tiles = 0;
+  for (int i = 0; i < p->n; ++i)
+    if (p->dw[i]) tiles += cdiv64(p->N[i], 128) * cdiv64(p->K[i], 128);
+  return splits_for(tiles, cdiv64(p->M, block_k(p->dtype)));
+}
+static bool dw_ok(const dpvo_gated_linear_dw_t* p) {
+  if (!p || p->n < 0 || p->n > MAXP || !type_ok(p->dtype) || p->M < 0) return false;
+  for (int i = 0; i < p->n; ++i) {
+    if (p->N[i] < 0 || p->K[i] < 0) return false;
+    if (!p->M || !p->N[i]) continue;
+    if (!p->a[i] || !ld_ok(p->lda[i], p->N[i], type_size(p->dtype))) return false;
+    if (p->dw[i] && p->K[i] && (!p->b[i] || !ld_ok(p->ldb[i], p->K[i], type_size(p->dtype)))) return false;
+  }
+  return true;
+}
+extern "C" size_t dpvo_gated_linear_dw_workspace_bytes(const dpvo_gated_linear_dw_t* p) {
+  if (!dw_ok(p)) return 0;
+  const int64_t s = dw_splits(p);
+  int64_t f = 0;
+  for (int i = 0; i < p->n; ++i) {
+    if (p->dw[i] && s > 1) f += s * p->N[i] * p->K[i];
+    if (p->db[i]) f += col_parts(p->M) * p->N[i];
+  }
+  return (size_t)f * 4;
+}
+extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, size_t ws_bytes, void* stream) {
+  if (!dw_ok(p)) return DPVO_E_INVALID;
+  if (dpvo_gated_linear_dw_workspace_bytes(p) > ws_bytes) return DPVO_E_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t splits = dw_splits(p);
+  float* w = (float*)ws;
+  GemmArgs a = {};
+  int64_t tiles = 0;
+  int which[MAXP];
+  for (int i = 0; i < p->n; ++i) {
+    if (!p->dw[i] || !p->N[i] || !p->K[i]) continue;
+    Prob& q = a.p[a.n];
+    which[a.n++] = i;
+    q.A[0] = p->a[i]; q.B[0] = p->b[i]; q.lda[0] = p->lda[i]; q.ldb[0] = p->ldb[i]; q.K[0] = p->M;
+    q.M = p->N[i]; q.N = p->K[i];
+    q.nb0 = q.nb = cdiv64(p->M, block_k(p->dtype));
+    q.splits = (int)splits;
+    q.out0 = p->dw[i]; q.ldo = p->K[i];
+    if (splits > 1) {
+      q.part = w;
+      w += splits * q.M * q.N;
+    }
+    tiles_of(q, 128, 128);
+    q.tile0 = tiles;
+    tiles += q.tm * q.tn * splits;
+  }
+  int rc = gemm(a, p->dtype, F_TN, E_LIN, 0, tiles, s);
+  if (rc) return rc;
+  if (splits > 1)
+    for (int i = 0; i < a.n; ++i)
+      if ((rc = split_sum(a.p[i].part, a.p[i].M * a.p[i].N, (int)splits, nullptr, p->dw[which[i]], p->dtype, s))) return rc;
+  ColArgs c = {};
+  int64_t width = 0;
+  for (int i = 0; i < p->n; ++i) {
+    if (!p->db[i] || !p->N[i]) continue;
+    ColJob& j = c.j[c.n++];
+    j.a = p->a[i]; j.lda = p->lda[i]; j.M = p->M; j.N = p->N[i]; j.part = w; j.out = p->db[i]; j.parts = col_parts(p->M); j.outs = 1; j.type = p->dtype;
+    w += j.parts * j.N;
+    width = j.N > width ? j.N : width;
+  }
+  if (c.n == 0) return DPVO_OK;
+  hipLaunchKernelGGL(col_sum_kernel, dim3((unsigned)cdiv64(width, 256), (unsigned)col_parts(p->M), (unsigned)c.n), dim3(256), 0, s, c);
+  DPVO_LAUNCH_CHECK();
+  return col_reduce(c, s);
+}
+
+extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {
+  const int rc = norm_check(p);
+  if (rc) return rc;
+  if (p->M == 0) return DPVO_OK;
+  if (p->ldx < p->D || (p->f && p->ldf < p->D) || (p->gate && p->ldgate < p->D) || (p->norm && !p->h) || (!p->norm && !p->s)) return DPVO_E_INVALID;
+  NormArgs a = {};
+  a.p = *p;
+  a.rows_per_gate = p->gate ? p->M / p->groups : 1;
+  const NormShape sh = norm_shape(p->D);
+  const int64_t want = cdiv64(p->M, norm_slots(sh));
+  return norm_run(a, sh, false, want < 8192 ? want : 8192, (hipStream_t)stream);
+}
+
+extern "C" size_t dpvo_residual_norm_backward_workspace_bytes(const dpvo_residual_norm_t* p) {
+  if (norm_check(p) || p->M == 0) return 0;
+  const NormPlan n = norm_plan(*p);
+  const int64_t rows = (n.shared ? n.groups * n.bpg : 0) + n.blocks * ((p->dw != nullptr) + (p->db != nullptr) + (p->dpw != nullptr) + (p->dpb != nullptr));
+  return (size_t)(rows * p->D * 4);
+}
+extern "C" int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* ws, size_t ws_bytes, void* stream) {
+  int rc = norm_check(p);
+  if (rc) return rc;
+  if (p->ldx < p->D || (p->f && p->ldf < p->D) || (p->gate && p->ldgate < p->D) || (p->ds && p->ldds < p->D) || (p->dh && p->lddh < p->D)) return DPVO_E_INVALID;
+  if ((!p->f && (p->df || p->dgate || p->dpw || p->dpb)) || (p->dgate && !p->gate) || (p->post == DPVO_NORM_NONE && (p->dpw || p->dpb))) return DPVO_E_INVALID;
+  if (dpvo_residual_norm_backward_workspace_bytes(p) > ws_bytes) return DPVO_E_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  NormArgs a = {};
+  a.p = *p;
+  ColArgs c = {};
+  float* w = (float*)ws;
+  const NormPlan n = p->M ? norm_plan(*p) : NormPlan{norm_shape(p->D), 0, 0, 1, 1, 0, false};
+  a.rows_per_gate = p->gate && p->M ? p->M / p->groups : 1;
+  a.groups = n.groups; a.rpg = n.rpg; a.gpb = n.gpb; a.bpg = n.bpg;
+  auto job = [&](void* out, int type, int64_t outs, int64_t parts) {
+    if (!out) return (float*)nullptr;
+    ColJob& j = c.j[c.n++];
+    j.part = w; j.out = out; j.type = type; j.N = p->D; j.outs = outs; j.parts = parts;
+    w += outs * parts * p->D;
+    return j.part;
+  };
+  a.part_w = job(p->dw, p->w_dtype, 1, n.blocks);
+  a.part_b = job(p->db, p->w_dtype, 1, n.blocks);
+  a.part_pw = job(p->dpw, p->w_dtype, 1, n.blocks);
+  a.part_pb = job(p->dpb, p->w_dtype, 1, n.blocks);
+  if (n.shared) a.part_gate = job(p->dgate, p->f_dtype, n.groups, n.bpg);
+  else if (!p->M && p->dgate) job(p->dgate, p->f_dtype, p->groups, 0);
+  if (p->M) {
+    rc = norm_run(a, n.sh, true, n.blocks, s);
+    if (rc) return rc;
+  }
+  return col_reduce(c, s);                               // (no rows: parts = 0, the shared gradients are zeros)
+}

@@ -35,10 +35,18 @@ extern "C" {
 
 #define DPVO_F16 0
 #define DPVO_F32 1
+#define DPVO_BF16 2              /* dpvo_gated_linear* and dpvo_residual_norm* only */
+
+#define DPVO_ACT_IDENTITY 0
+#define DPVO_ACT_RELU 1
+#define DPVO_ACT_SIGMOID 2
+#define DPVO_ACT_SILU 3
+#define DPVO_ACT_GELU 4          /* z/2 (1 + erf(z / sqrt 2))                                  */
+#define DPVO_ACT_GELU_TANH 5     /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))              */
 
 /* ABI version: bumped on ANY change of a signature, a struct layout or the exported set (round 3 changed all three without a
  * bump).  The Python binding refuses a library whose version differs from the one it was written against. */
-#define DPVO_ABI_VERSION 8
+#define DPVO_ABI_VERSION 9
 int dpvo_abi_version(void);
 
 /* ------------------------------------------------------------------------------------------------
@@ -569,6 +577,81 @@ int dpvo_solve_system(const float* J_Ginv_i, const float* J_Ginv_j, const int64_
 /* Dev aid: a one-thread kernel that stores the 100 MHz wall clock into *slot (uint64) when it executes: stream-ordered time
  * stamps across streams without a profiler (tools/stream_stamps.py). */
 int dpvo_debug_stamp(void* slot, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Gated feed-forward blocks and the norms around them, forward and backward (dpvo_amd/blocks.py; the reference's GatedResidual and
+ * LayerNorms are dpvo/blocks.py:15-48 and dpvo/net.py:44-59, trained through torch autograd).
+ * Types: DPVO_F16, DPVO_BF16 or DPVO_F32 operands, all sums and activations in f32.  Rows may start at any element (a leading dimension
+ * need not be a multiple of anything); a row's elements are contiguous.  Any size from 0 up, limited only where stated.  Nothing is
+ * accumulated atomically: results do not vary from run to run.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* y = act(x w_gate^T + b_gate) [* (v w_up^T + b_up)] [+ residual]
+ *   x [M,K], w_gate [N,K]; with w_up [N,Kv]: v [M,Kv] (v == x and Kv == K, or another input); b_gate, b_up [N], residual [M,N] or NULL;
+ *   y [M,N]; save_gate / save_up [M,N] f32 contiguous or NULL: the two sums before the activation, for dpvo_gated_linear_dact.
+ *   Leading dimensions in elements; ld * 256 * element size < 2^31. */
+typedef struct {
+  const void *x, *v, *w_gate, *w_up, *b_gate, *b_up, *residual;
+  void* y;
+  float *save_gate, *save_up;
+  int64_t ldx, ldv, ldwg, ldwu, ldr, ldy;
+  int64_t M, N, K, Kv;
+  int32_t dtype, activation;
+} dpvo_gated_linear_t;
+int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream);
+
+/* Gradients of the two sums from dy [M,N] (leading dimension lddy): d_gate = dy * up * act'(gate), d_up = dy * act(gate), both [M,N] with
+ * leading dimension ldo in `dtype`; up == NULL (no product): d_gate = dy * act'(gate) alone.  gate, up: f32 contiguous, as saved. */
+int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, const float* up, void* d_gate, void* d_up, int64_t ldo,
+                           int dtype, int activation, int64_t M, int64_t N, void* stream);
+
+/* Input gradient dx [M,N] = a0 b0 [+ a1 b1] [+ addend]: a_s [M,K_s] gradients of the sums, b_s [K_s,N] the weights as stored.
+ * With `gate` (f32 [M,N] contiguous, as saved) dx is itself the gradient of act(gate) [* up] and is taken through it at once:
+ * dx = d_gate, dx2 = d_up as in dpvo_gated_linear_dact; with `mask` [M,N] (the ReLU's output) dx is kept where mask > 0.
+ * addend is allowed with neither.  ws: dpvo_gated_linear_dx_workspace_bytes(M, N, K0 + K1) bytes (0 when few parts are needed). */
+typedef struct {
+  const void *a[2], *b[2], *addend, *mask;
+  const float *gate, *up;
+  void *dx, *dx2;
+  int64_t lda[2], ldb[2], K[2], ldadd, ldmask, lddx;
+  int64_t M, N;
+  int32_t dtype, activation;
+} dpvo_gated_linear_dx_t;
+size_t dpvo_gated_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, size_t ws_bytes, void* stream);
+
+/* Weight gradients, up to four at once: dw_i [N_i,K_i] = a_i^T b_i over the M rows of a_i [M,N_i] (gradient of a sum) and b_i [M,K_i] (its
+ * input); db_i [N_i] = column sums of a_i (or NULL).  dw_i contiguous; dw_i == NULL: only db_i. */
+typedef struct {
+  const void *a[4], *b[4];
+  void *dw[4], *db[4];
+  int64_t lda[4], ldb[4], N[4], K[4];
+  int64_t M;
+  int32_t n, dtype;
+} dpvo_gated_linear_dw_t;
+size_t dpvo_gated_linear_dw_workspace_bytes(const dpvo_gated_linear_dw_t* p);
+int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, size_t ws_bytes, void* stream);
+
+/* s = x + scale * act(gate) * post(f);  h = norm(s).   Norms: LAYER (x - mean) / sqrt(var + eps) * w + b, RMS x / sqrt(mean x^2 + eps) * w + b.
+ *   x, s [M,D] in x_dtype; f [M,D] and gate [groups,D] in f_dtype (f == NULL: s = x; gate == NULL: no factor; row m reads gate row
+ *   m / (M / groups)); w, b, pw, pb [D] in w_dtype or NULL; h [M,D] in h_dtype, x_dtype or f_dtype; s, h contiguous; s may be NULL.
+ *   x_dtype is f_dtype or DPVO_F32.  1 <= D <= 16384.  norm == NONE: h is not written.
+ * backward: ds, dh (NULL: zero) -> dx (x_dtype), df, dgate (f_dtype), dw, db, dpw, dpb (w_dtype), each NULL if not wanted, contiguous. */
+#define DPVO_NORM_NONE 0
+#define DPVO_NORM_LAYER 1
+#define DPVO_NORM_RMS 2
+typedef struct {
+  const void *x, *f, *gate, *w, *b, *pw, *pb;
+  void *s, *h;
+  const void *ds, *dh;
+  void *dx, *df, *dgate, *dw, *db, *dpw, *dpb;
+  int64_t ldx, ldf, ldgate, ldds, lddh, M, groups;
+  int32_t D, x_dtype, f_dtype, h_dtype, w_dtype, norm, post, gate_activation;
+  float scale, eps, post_eps;
+} dpvo_residual_norm_t;
+int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream);
+size_t dpvo_residual_norm_backward_workspace_bytes(const dpvo_residual_norm_t* p);
+int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
