@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from . import _lib as L
 from . import workspace
 from . import altcorr
+from . import blocks
 from .extractor import BasicEncoder4
 from .graph import GraphPlan
 from .utils import coords_grid_with_index
@@ -134,6 +135,22 @@ class GatedResidual(nn.Module):
         self.gate = nn.Sequential(nn.Linear(dim, dim), nn.Sigmoid())
         self.res = nn.Sequential(nn.Linear(dim, dim), nn.ReLU(inplace=True), nn.Linear(dim, dim))
 
+    def forward(self, x):
+        """x + gate(x) * res(x) (dpvo/blocks.py:23-24), differentiable; runs in x's dtype (f32 as the reference trains, or f16 / bf16)"""
+        gate, first, last = self.gate[0], self.res[0], self.res[2]
+        to = lambda t: t.to(x.dtype)
+        return blocks.gated_residual(x, to(gate.weight), to(gate.bias), to(first.weight), to(first.bias), to(last.weight), to(last.bias))
+
+
+class GatedStack(nn.Sequential):
+    """LayerNorm, GatedResidual, LayerNorm, GatedResidual (net.py:44-49: Update.gru), differentiable: `update.gru(net)` trains or fine-tunes
+    this stage on its own.  The tracker does not come by here: Update.forward runs the stage inside its seven kernels."""
+
+    def forward(self, x):
+        for m in self:
+            x = blocks.norm(x, m.weight, m.bias, "layer", m.eps) if isinstance(m, nn.LayerNorm) else m(x)
+        return x
+
 
 class SoftAgg(nn.Module):
     def __init__(self, dim=512, expand=True):
@@ -153,7 +170,7 @@ class Update(nn.Module):
         self.norm = nn.LayerNorm(DIM, eps=1e-3)
         self.agg_kk = SoftAgg(DIM)
         self.agg_ij = SoftAgg(DIM)
-        self.gru = nn.Sequential(
+        self.gru = GatedStack(
             nn.LayerNorm(DIM, eps=1e-3), GatedResidual(DIM),
             nn.LayerNorm(DIM, eps=1e-3), GatedResidual(DIM))
         self.corr = nn.Sequential(

@@ -389,3 +389,72 @@ def residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, us
 def test_residual_norm(dev, tx, tb, lead, D, kind, post, gate, gate_act, scale, use):
     g = torch.Generator().manual_seed(D + len(lead))
     residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, use)
+
+
+# ------------------------------------------------------------------------------------------------------------------ together, as the model has them
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_update_gru(dev, t):
+    """Update.gru (LayerNorm, gated residual block, twice) and its gradients, through the model's own module, against the carried bounds"""
+    from dpvo_amd import net as N
+    torch.manual_seed(3)
+    gru = N.Update(3).gru.to(dev)
+    with torch.no_grad():
+        for p in gru.parameters():
+            if p.dim() == 1:
+                p.add_(0.05 * torch.randn_like(p))
+    g = torch.Generator().manual_seed(8)
+    x = make(g, 1, 150, 384, t=t)
+    dy = make(g, 1, 150, 384, t=t, grad=False)
+    y = gru(x)
+    grads = torch.autograd.grad(y, [x, *gru.parameters()], dy)
+    names = ["x"] + [n for n, _ in gru.named_parameters()]
+    par = {n: p for n, p in gru.named_parameters()}
+    op = lambda n: V(par[n].detach().to(t).double().cpu())  # noqa: E731
+    full = lambda n: rows_f(par[n])  # noqa: E731
+    z, kept = rows_f(x[0]), []
+    for i in (0, 2):
+        xh, r = normalise(z, "layer", 1e-3)
+        h = (xh * full(f"{i}.weight") + full(f"{i}.bias")).to(t)
+        q = f"{i + 1}."
+        a, d1 = act("relu", proj(h, op(q + "res.0.weight"), op(q + "res.0.bias")))
+        a = a.to(t)
+        out, G, R, ya, da = gated_reference(h, op(q + "gate.0.weight"), op(q + "res.2.weight"), op(q + "gate.0.bias"), op(q + "res.2.bias"), "sigmoid", a, h)
+        kept.append((xh, r, h, a, d1, R, ya, da))
+        z = out.to(t)
+    within(y, z, t, "y")
+    want, D = {}, rows_f(dy[0])
+    for i in (2, 0):
+        xh, r, h, a, d1, R, ya, da = kept[i // 2]
+        q = f"{i + 1}."
+        dg, dr = (D * R * da).to(t), (D * ya).to(t)
+        dp = (dr.mm(op(q + "res.2.weight")) * d1).to(t)
+        for n, u, v in (("gate.0", dg, h), ("res.0", dp, h), ("res.2", dr, a)):
+            want[q + n + ".weight"], want[q + n + ".bias"] = u.t().mm(v).to(t), u.sum0().to(t)
+        D = (dg.mm(op(q + "gate.0.weight")) + dp.mm(op(q + "res.0.weight")) + D).to(t)
+        want[f"{i}.weight"], want[f"{i}.bias"] = (D * xh).sum0(), D.sum0()
+        D = norm_back(D * full(f"{i}.weight"), xh, r, "layer").to(t)
+    want["x"] = D
+    for n, got in zip(names, grads):
+        within(got, want[n], got.dtype, n)
+
+
+def test_gru_is_the_stage_of_the_tracker(dev):
+    """the same stage in Update.forward's comparator pieces (launch by launch, f16 operands, f32 state) and here in f16: each is within the
+    roundings of its f16 operands of the other"""
+    from dpvo_amd import net as N
+    torch.manual_seed(4)
+    upd = N.Update(3).to(dev)
+    x = torch.randn(1, 200, 384, generator=torch.Generator().manual_seed(1)).cuda()
+    with torch.no_grad():
+        y = upd.gru(x)
+        P = upd.pack()
+        z = x[0].clone()
+        h1 = torch.empty(200, 384, dtype=F16, device=dev)
+        fg = torch.empty(200, 768, dtype=F16, device=dev)
+        for name in ("g0", "g1"):
+            gm, b, Wrg, brg, W2, b2 = P[name]
+            N.layernorm(z, gm, b, y_f32=z, y_f16=h1)
+            N.linear(h1, Wrg, brg, out=fg, epilogue=N.EPI_RELU_SIG, n_split=384)
+            N.linear(fg[:, :384], W2, b2, out=z, epilogue=N.EPI_GATED, gate=fg[:, 384:])
+    # roundings per block: operand h, weights, the hidden layer, the gate, twice over; each half a step (2^-11) of values of a few units
+    assert float((y[0] - z).abs().max()) < 16 * 2.0 ** -11 * float(z.abs().max())
