@@ -158,8 +158,7 @@ def lib():
         vp, i64_, i32_ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
         L.dpvo_gated_linear.argtypes = [vp, vp]
         L.dpvo_gated_linear_dact.argtypes = [vp, i64_, vp, vp, vp, vp, i64_, i32_, i32_, i64_, i64_, vp]
-        L.dpvo_gated_linear_dx_workspace_bytes.argtypes = [i64_, i64_, i64_]
-        L.dpvo_gated_linear_dw_workspace_bytes.argtypes = L.dpvo_residual_norm_backward_workspace_bytes.argtypes = [vp]
+        L.dpvo_gated_linear_dx_workspace_bytes.argtypes = L.dpvo_gated_linear_dw_workspace_bytes.argtypes = L.dpvo_residual_norm_backward_workspace_bytes.argtypes = [vp]
         L.dpvo_gated_linear_dx.argtypes = L.dpvo_gated_linear_dw.argtypes = L.dpvo_residual_norm_backward.argtypes = [vp, vp, ctypes.c_size_t, vp]
         L.dpvo_residual_norm.argtypes = [vp, vp]
         L.dpvo_abi_version.restype = ctypes.c_int

@@ -163,7 +163,7 @@ def _dx(pairs, addend=None, gate=None, up=None, mask=None, act=0):
     p.addend, p.mask, p.gate, p.up, p.dx, p.dx2 = _p(addend), _p(mask), _p(gate), _p(up), _p(dx), _p(dx2)
     p.lddx, p.M, p.N, p.dtype, p.activation = N, M, N, _DTYPES[ref.dtype], act
     lib = L.lib()
-    n = 0 if gate is not None or mask is not None else lib.dpvo_gated_linear_dx_workspace_bytes(M, N, sum(a.shape[1] for a in keep[::2]))
+    n = lib.dpvo_gated_linear_dx_workspace_bytes(ctypes.byref(p))
     ws = _scratch(n, ref.device)
     L.check(lib.dpvo_gated_linear_dx(ctypes.byref(p), _p(ws), n, L.stream()), "dpvo_gated_linear_dx")
     return dx, dx2

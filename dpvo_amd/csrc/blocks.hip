@@ -13,22 +13,13 @@ inline bool act_ok(int a) { return a >= DPVO_ACT_IDENTITY && a <= DPVO_ACT_GELU_
 // row offsets within a tile are 32-bit bytes
 inline bool ld_ok(int64_t ld, int64_t width, int size) { return ld >= width && ld <= INT_MAX / (256 * size); }
 
-int gemm(const GemmArgs& a, int dtype, int form, int epi, int big, int64_t tiles, hipStream_t s) {
+int gemm(const GemmArgs& a, int dtype, int form, int epi, int kind, int64_t tiles, hipStream_t s) {
   if (tiles > INT_MAX) return DPVO_E_UNSUPPORTED;
-  if (dtype == DPVO_F16) return gemm_f16(a, form, epi, big, tiles, s);
-  if (dtype == DPVO_BF16) return gemm_bf16(a, form, epi, big, tiles, s);
-  return gemm_f32(a, form, epi, big, tiles, s);
+  if (dtype == DPVO_F16) return gemm_f16(a, form, epi, kind, tiles, s);
+  if (dtype == DPVO_BF16) return gemm_bf16(a, form, epi, kind, tiles, s);
+  return gemm_f32(a, form, epi, kind, tiles, s);
 }
 inline int block_k(int dtype) { return dtype == DPVO_F32 ? 32 : 64; }
-
-// Parts a sum over `nb` blocks is cut into when its `tiles` tiles are too few for the chip: two workgroups on each of 256 compute units, but at
-// least 8 blocks to a part (a part costs a tile's write and read in f32).
-int64_t splits_for(int64_t tiles, int64_t nb) {
-  if (tiles <= 0) return 1;
-  int64_t s = 512 / tiles;
-  if (s > nb / 8) s = nb / 8;
-  return s < 1 ? 1 : s > 64 ? 64 : s;
-}
 
 // out[e] = sum over splits of part[split][e] (+ addend[e]), all contiguous
 template <class T> __global__ void __launch_bounds__(256) split_sum_kernel(const float* part, int64_t size, int splits, const T* addend, T* out) {
@@ -71,7 +62,7 @@ template <class T> __global__ void __launch_bounds__(256) dact_kernel(const T* d
     load_n<float, 8>(gate + m * N + n, nv, g);
     if (up) load_n<float, 8>(up + m * N + n, nv, u);
     float o[8];
-    act_d8<sizeof(T) == 4>(act, g, o);
+    act_d_n<sizeof(T) == 4>(act, g, o);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       o[e] *= d[e];
@@ -163,9 +154,35 @@ int col_reduce(const ColArgs& c, hipStream_t s) {
 }
 int64_t col_parts(int64_t M) { return M < 64 ? 1 : M / 64 < 256 ? M / 64 : 256; }
 
-void tiles_of(Prob& p, int tm, int tn) {
-  p.tm = cdiv64(p.M, tm);
-  p.tn = cdiv64(p.N, tn);
+// ---- which tiles, and in how many parts the summed index is cut where there are too few of them
+struct Plan {
+  int kind;
+  int64_t splits;
+};
+inline int tile_size(int kind) { return kind == T_BIG ? 256 : kind == T_SMALL ? 64 : 128; }
+// `count(t)`: tiles of t x t; nb: blocks of the summed index; cut: whether parts are possible.
+// 256 x 256 reads LDS least per product and gives 1095 Tflop/s (bf16, 8192 x 8192 x 4096) where 128 x 128 gives 885; but only one workgroup
+// fits a compute unit, so its epilogue hides behind nothing: with 16 blocks it still wins (79.7 against 89.3 us, 4096 x 4096 x 1024 twice),
+// with 6 it loses (65.2 against 56.6 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
+// 128 x 128 wants two workgroups on a compute unit: at 432 tiles it wins over 64 x 64 (15.7 against 20.6 us), at 256 it loses (19.1 against 18.0).
+template <class F> Plan plan(F count, int64_t nb, int dtype, bool cut) {
+  if (dtype != DPVO_F32 && nb >= 12 && count(256) >= 200) return {T_BIG, 1};
+  const int64_t t = count(128);
+  if (t >= 384) return {T_TILE, 1};
+  if (cut && t > 0) {
+    int64_t s = 512 / t;
+    if (s > nb / 8) s = nb / 8;
+    if (s > 64) s = 64;
+    if (s > 1) return {T_TILE, s};
+  }
+  return {T_SMALL, 1};
+}
+inline int64_t tiles(int64_t M, int64_t N, int t) { return cdiv64(M, t) * cdiv64(N, t); }
+int64_t tiles_of(Prob& p, int kind, int halves = 1) {
+  const int t = tile_size(kind);
+  p.tm = cdiv64(p.M, t);
+  p.tn = cdiv64(p.N, t / halves);
+  return p.tm * p.tn;
 }
 
 // ---- the norm backward's share of rows
@@ -235,8 +252,11 @@ extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream) {
   const int bk = block_k(p->dtype), epi = !p->w_up ? E_LIN : same ? E_GATE : E_GATE2;
   q.nb0 = cdiv64(p->K, bk);
   q.nb = q.nb0 + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0);
-  tiles_of(q, 128, epi == E_GATE ? 64 : 128);
-  return gemm(a, p->dtype, F_NT, epi, 0, q.tm * q.tn, (hipStream_t)stream);
+  if (p->M <= FEW_ROWS) return gemm(a, p->dtype, F_NT, epi, T_FEW, cdiv64(p->N, 16), (hipStream_t)stream);
+  int kind = plan([&](int t) { return tiles(p->M, epi == E_GATE ? 2 * p->N : p->N, t); }, q.nb, p->dtype, false).kind;
+  if (epi == E_GATE2 && kind == T_BIG) kind = T_TILE;    // (two sets of sums do not fit the registers of the largest tile)
+  const int64_t n = tiles_of(q, kind, epi == E_GATE ? 2 : 1);
+  return gemm(a, p->dtype, F_NT, epi, kind, n, (hipStream_t)stream);
 }
 
 extern "C" int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, const float* up, void* d_gate, void* d_up, int64_t ldo, int dtype,
@@ -253,13 +273,14 @@ extern "C" int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float*
   return DPVO_OK;
 }
 
-// (the workspace does not know the type: blocks of 32 are the finer cut)
-static int64_t dx_splits(int64_t M, int64_t N, int64_t K, int bk) { return splits_for(cdiv64(M, 128) * cdiv64(N, 128), cdiv64(K, bk)); }
+static Plan dx_plan(int64_t M, int64_t N, int64_t nb, int dtype, bool cut) { return plan([&](int t) { return tiles(M, N, t); }, nb, dtype, cut); }
 
-extern "C" size_t dpvo_gated_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const int64_t s = dx_splits(M, N, K + 64, 32);
-  return s > 1 ? (size_t)(s * M * N * 4) : 0;
+extern "C" size_t dpvo_gated_linear_dx_workspace_bytes(const dpvo_gated_linear_dx_t* p) {
+  if (!p || !type_ok(p->dtype) || p->M <= 0 || p->N <= 0 || p->K[0] < 0 || p->K[1] < 0 || p->gate || p->mask) return 0;
+  if (p->lddx != p->N || (p->addend && p->ldadd != p->N)) return 0;
+  const int bk = block_k(p->dtype);
+  const Plan c = dx_plan(p->M, p->N, cdiv64(p->K[0], bk) + (p->a[1] ? cdiv64(p->K[1], bk) : 0), p->dtype, true);
+  return c.splits > 1 ? (size_t)(c.splits * p->M * p->N * 4) : 0;
 }
 
 extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, size_t ws_bytes, void* stream) {
@@ -287,32 +308,36 @@ extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, s
   q.nb0 = cdiv64(p->K[0], bk);
   q.nb = q.nb0 + cdiv64(K1, bk);
   q.splits = 1;
-  tiles_of(q, 128, 128);
   hipStream_t s = (hipStream_t)stream;
   if (p->gate || p->mask) {
+    const int kind = dx_plan(p->M, p->N, q.nb, p->dtype, false).kind;
+    tiles_of(q, kind);
     q.save0 = (float*)p->gate; q.save1 = (float*)p->up; q.mask = p->mask; q.ldmask = p->ldmask;
-    return gemm(a, p->dtype, F_NN, E_DACT, 0, q.tm * q.tn, s);
+    return gemm(a, p->dtype, F_NN, E_DACT, kind, q.tm * q.tn, s);
   }
   q.act = DPVO_ACT_IDENTITY;
   const bool flat = p->lddx == p->N && (!p->addend || p->ldadd == p->N);
-  const int64_t splits = flat ? splits_for(q.tm * q.tn, q.nb) : 1;
-  if (splits > 1) {
-    if ((size_t)(splits * p->M * p->N * 4) > ws_bytes || !ws) return DPVO_E_WORKSPACE;
-    q.splits = (int)splits;
+  const Plan c = dx_plan(p->M, p->N, q.nb, p->dtype, flat);
+  tiles_of(q, c.kind);
+  if (c.splits > 1) {
+    if ((size_t)(c.splits * p->M * p->N * 4) > ws_bytes || !ws) return DPVO_E_WORKSPACE;
+    q.splits = (int)c.splits;
     q.part = (float*)ws;
-    const int rc = gemm(a, p->dtype, F_NN, E_LIN, 0, q.tm * q.tn * splits, s);
+    const int rc = gemm(a, p->dtype, F_NN, E_LIN, c.kind, q.tm * q.tn * c.splits, s);
     return rc ? rc : split_sum(q.part, p->M * p->N, q.splits, p->addend, p->dx, p->dtype, s);
   }
   q.addend = p->addend; q.ldadd = p->ldadd;
-  return gemm(a, p->dtype, F_NN, E_LIN, 0, q.tm * q.tn, s);
+  return gemm(a, p->dtype, F_NN, E_LIN, c.kind, q.tm * q.tn, s);
 }
 
 // workspace: the parts of each product that is split, then the partial column sums
-static int64_t dw_splits(const dpvo_gated_linear_dw_t* p) {
-  int64_t tiles = 0;
-  for (int i = 0; i < p->n; ++i)
-    if (p->dw[i]) tiles += cdiv64(p->N[i], 128) * cdiv64(p->K[i], 128);
-  return splits_for(tiles, cdiv64(p->M, block_k(p->dtype)));
+static Plan dw_plan(const dpvo_gated_linear_dw_t* p) {
+  return plan([&](int t) {
+    int64_t n = 0;
+    for (int i = 0; i < p->n; ++i)
+      if (p->dw[i]) n += tiles(p->N[i], p->K[i], t);
+    return n;
+  }, cdiv64(p->M, block_k(p->dtype)), p->dtype, true);
 }
 static bool dw_ok(const dpvo_gated_linear_dw_t* p) {
   if (!p || p->n < 0 || p->n > MAXP || !type_ok(p->dtype) || p->M < 0) return false;
@@ -326,7 +351,7 @@ static bool dw_ok(const dpvo_gated_linear_dw_t* p) {
 }
 extern "C" size_t dpvo_gated_linear_dw_workspace_bytes(const dpvo_gated_linear_dw_t* p) {
   if (!dw_ok(p)) return 0;
-  const int64_t s = dw_splits(p);
+  const int64_t s = dw_plan(p).splits;
   int64_t f = 0;
   for (int i = 0; i < p->n; ++i) {
     if (p->dw[i] && s > 1) f += s * p->N[i] * p->K[i];
@@ -338,10 +363,11 @@ extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, s
   if (!dw_ok(p)) return DPVO_E_INVALID;
   if (dpvo_gated_linear_dw_workspace_bytes(p) > ws_bytes) return DPVO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t splits = dw_splits(p);
+  const Plan c0 = dw_plan(p);
+  const int64_t splits = c0.splits;
   float* w = (float*)ws;
   GemmArgs a = {};
-  int64_t tiles = 0;
+  int64_t n = 0;
   int which[MAXP];
   for (int i = 0; i < p->n; ++i) {
     if (!p->dw[i] || !p->N[i] || !p->K[i]) continue;
@@ -356,11 +382,10 @@ extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, s
       q.part = w;
       w += splits * q.M * q.N;
     }
-    tiles_of(q, 128, 128);
-    q.tile0 = tiles;
-    tiles += q.tm * q.tn * splits;
+    q.tile0 = n;
+    n += tiles_of(q, c0.kind) * splits;
   }
-  int rc = gemm(a, p->dtype, F_TN, E_LIN, 0, tiles, s);
+  int rc = gemm(a, p->dtype, F_TN, E_LIN, c0.kind, n, s);
   if (rc) return rc;
   if (splits > 1)
     for (int i = 0; i < a.n; ++i)

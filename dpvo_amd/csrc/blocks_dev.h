@@ -84,9 +84,9 @@ template <bool FINE> __device__ __forceinline__ ActD act_d(int a, float z) {
   }
 }
 
-// eight at a time, the choice outside
-template <bool FINE> __device__ __forceinline__ void act8(int a, float (&v)[8]) {
-#define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] = act_<FINE>(A, v[e]); return;
+// N at a time, the choice outside
+template <bool FINE, int N> __device__ __forceinline__ void act_n(int a, float (&v)[N]) {
+#define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] = act_<FINE>(A, v[e]); return;
   switch (a) {
     BLK_CASE(DPVO_ACT_RELU)
     BLK_CASE(DPVO_ACT_SIGMOID)
@@ -97,8 +97,8 @@ template <bool FINE> __device__ __forceinline__ void act8(int a, float (&v)[8]) 
 #undef BLK_CASE
 }
 // z -> value y and derivative (in z)
-template <bool FINE> __device__ __forceinline__ void act_d8(int a, float (&z)[8], float (&y)[8]) {
-#define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < 8; ++e) { const ActD t = act_d<FINE>(A, z[e]); y[e] = t.y; z[e] = t.d; } return;
+template <bool FINE, int N> __device__ __forceinline__ void act_d_n(int a, float (&z)[N], float (&y)[N]) {
+#define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < N; ++e) { const ActD t = act_d<FINE>(A, z[e]); y[e] = t.y; z[e] = t.d; } return;
   switch (a) {
     BLK_CASE(DPVO_ACT_RELU)
     BLK_CASE(DPVO_ACT_SIGMOID)
@@ -138,8 +138,12 @@ struct GemmArgs {
   int n;
 };
 
-int gemm_f16(const GemmArgs& a, int form, int epi, int big, int64_t tiles, hipStream_t s);
-int gemm_bf16(const GemmArgs& a, int form, int epi, int big, int64_t tiles, hipStream_t s);
-int gemm_f32(const GemmArgs& a, int form, int epi, int big, int64_t tiles, hipStream_t s);
+// how a product is run: tiles of 128 x 128, 256 x 256 or 64 x 64, or few rows with the summed index over the waves (blocks_gemm.h)
+enum { T_TILE = 0, T_BIG = 1, T_SMALL = 2, T_FEW = 3 };
+constexpr int FEW_ROWS = 64;
+
+int gemm_f16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);
+int gemm_bf16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);
+int gemm_f32(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);
 
 }  // namespace blk

@@ -13,6 +13,8 @@
 #pragma once
 #include "blocks_dev.h"
 
+#define BLK_INLINE __attribute__((always_inline))
+
 namespace blk {
 namespace {
 
@@ -21,9 +23,10 @@ constexpr int KE = Type<T>::KE;
 constexpr int BK = 8 * KE;
 constexpr bool FINE = sizeof(T) == 4;
 
-template <int BIG> struct Cfg;
-template <> struct Cfg<0> { static constexpr int NT = 256, TM = 128, TN = 128, WN = 2, MI = 2; };
-template <> struct Cfg<1> { static constexpr int NT = 512, TM = 256, TN = 256, WN = 4, MI = 4; };
+template <int KIND> struct Cfg;
+template <> struct Cfg<T_TILE> { static constexpr int NT = 256, TM = 128, TN = 128, WN = 2, MI = 2; };
+template <> struct Cfg<T_BIG> { static constexpr int NT = 512, TM = 256, TN = 256, WN = 4, MI = 4; };
+template <> struct Cfg<T_SMALL> { static constexpr int NT = 128, TM = 64, TN = 64, WN = 1, MI = 1; };
 
 __device__ __forceinline__ int swz(int row, int c) { return row * 128 + ((c ^ (row & 7) ^ ((row >> 3) & 7)) << 4); }
 
@@ -50,58 +53,88 @@ template <int N> __device__ __forceinline__ void raw_guard(const T* p, int64_t n
   }
 }
 
-// One operand's share of a tile: R rows x one block, by NT threads, four 16-byte pieces of registers each
+// One operand's share of a tile: R rows x one block, by NT threads, four 16-byte pieces of registers each.
+//   summed index contiguous (row): chunk t % 8 of rows t / 8 + i * NT / 8
+//   summed index as rows (col): columns 4 (t % (R / 4)) .. + 3 of summed indices KE (t / (R / 4)) .. + KE - 1
+// Whole blocks are loaded through a buffer descriptor whose base moves on (scalar work only) and per-lane offsets that never change;
+// a segment's last blocks through guarded loads.
 template <int R, int NT, bool TR> struct Stage {
   i4v v[4];
   static_assert(R * 8 == NT * 4, "four chunks per thread");
-  // summed index contiguous: chunk c of row (t / 8 + i * NT / 8).  `at(row)`: the row's element offset from the (uniform) base.
-  // summed index as rows: thread = (column group of 4, group of KE k)
-  uint32_t off[TR ? 1 : 4];
-  int c;
+  static constexpr int RS = NT / 8;                      // rows between a thread's chunks
+  uint32_t off[TR ? 1 : 4];                              // bytes from the tile's base
+  // where the pieces go in the first buffer: rows 64 apart have their chunks alike
+  static constexpr int NL = TR || RS == 16 ? 4 : RS == 32 ? 2 : 1;
+  uint32_t lds[NL];
 
-  template <class F> __device__ __forceinline__ void init(F at) {
-    const int t = threadIdx.x;
-    if constexpr (!TR) {
-      c = t & 7;
+  static __device__ __forceinline__ int chunk() { return TR ? (int)threadIdx.x / (R / 4) : (int)threadIdx.x & 7; }
+  static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x >> 3) + i * RS; }
+  static __device__ __forceinline__ int col() { return (int)threadIdx.x % (R / 4) * 4; }
+
+  __device__ __forceinline__ void init_lds(uint32_t base) {
+    if constexpr (TR) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) off[i] = (uint32_t)((at((t >> 3) + i * (NT / 8)) + c * KE) * (int64_t)sizeof(T));
+      for (int j = 0; j < 4; ++j) lds[j] = base + swz(col() + j, chunk());
     } else {
-      c = t / (R / 4);
-      off[0] = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) lds[i] = base + swz(row(i), chunk());
     }
   }
-  // `base`: element (row0, k) of the operand, uniform; nk: elements of the summed index from k on
-  __device__ __forceinline__ void load_row(const T* base) {
+  // row: `at(r)`: element offset of tile row r (clamped to the operand); col: `left`: columns from the tile's first on
+  template <class F> __device__ __forceinline__ void aim_rows(F at) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = ld_any<i4v>((const char*)base + off[i]);
+    for (int i = 0; i < 4; ++i) off[i] = (uint32_t)((at(row(i)) + chunk() * KE) * (int64_t)sizeof(T));
   }
-  __device__ __forceinline__ void load_row_guard(const T* base, int64_t nk) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      T o[KE];
-      raw_guard<KE>((const T*)((const char*)base + off[i]), nk - c * KE, o);
-      v[i] = __builtin_bit_cast(i4v, o);
-    }
+  __device__ __forceinline__ void aim_cols(int64_t ld, int64_t left) {
+    const int64_t last = (left - 1) / 4 * 4;             // groups behind the last column: the last group again, not stored
+    off[0] = (uint32_t)((chunk() * KE * ld + (col() < last ? col() : last)) * (int64_t)sizeof(T));
   }
-  // `base`: element (k, col0); cols: columns from col0 on
-  template <bool GUARD> __device__ __forceinline__ void load_col(const T* base, int64_t ld, int64_t nk, int64_t cols) {
-    const int cg = threadIdx.x % (R / 4);
-    const T* p = base + (int64_t)c * KE * ld + cg * 4;
-    T o[KE][4];
-#pragma unroll
-    for (int k = 0; k < KE; ++k) {
-      if constexpr (GUARD) raw_guard<4>(p + k * ld, c * KE + k < nk ? cols - cg * 4 : 0, o[k]);
-      else __builtin_memcpy(o[k], p + k * ld, sizeof(o[k]));
-    }
-    __builtin_memcpy(v, o, sizeof(v));
-  }
-  __device__ __forceinline__ void store(char* lds) const {
+  // base: (tile's first row, k), or for the pieces whose bit is set in `other` base1; col: (k, first column).  All scalar.
+  __device__ __forceinline__ void load(const T* base, const T* base1, int other, int64_t ld) {
     if constexpr (!TR) {
-      const int r = threadIdx.x >> 3;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *(i4v*)(lds + swz(r + i * (NT / 8), c)) = v[i];
+      for (int i = 0; i < 4; ++i) {
+        const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)(other >> i & 1 ? base1 : base), 0, -1, 0x27000);
+        v[i] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(d, off[i], 0, 0));
+      }
     } else {
-      const int cg = threadIdx.x % (R / 4);
+      const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
+      const uint32_t step = (uint32_t)(ld * sizeof(T));
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(d, off[0], k * step, 0));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                    // rows 2k, 2k + 1 of the 8 x 4 piece
+          const i2v lo = __builtin_bit_cast(i2v, __builtin_amdgcn_raw_buffer_load_b64(d, off[0], 2 * k * step, 0));
+          const i2v hi = __builtin_bit_cast(i2v, __builtin_amdgcn_raw_buffer_load_b64(d, off[0], (2 * k + 1) * step, 0));
+          v[k] = i4v{lo[0], lo[1], hi[0], hi[1]};
+        }
+      }
+    }
+  }
+  // the same with zeros for summed indices >= nk (counted from the block's first) and nothing read behind the operand
+  __device__ __forceinline__ void load_guard(const T* base, const T* base1, int other, int64_t ld, int64_t nk, int64_t left) {
+    if constexpr (!TR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        T o[KE];
+        raw_guard<KE>((const T*)((const char*)(other >> i & 1 ? base1 : base) + off[i]), nk - chunk() * KE, o);
+        v[i] = __builtin_bit_cast(i4v, o);
+      }
+    } else {
+      const T* p = base + (int64_t)chunk() * KE * ld + col();
+      T o[KE][4];
+#pragma unroll
+      for (int k = 0; k < KE; ++k) raw_guard<4>(p + k * ld, chunk() * KE + k < nk ? left - col() : 0, o[k]);
+      __builtin_memcpy(v, o, sizeof(v));
+    }
+  }
+  __device__ __forceinline__ void store(char* buf, uint32_t flip) const {
+    if constexpr (!TR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *(i4v*)(buf + ((lds[i % NL] + i / NL * NL * RS * 128) ^ flip)) = v[i];
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         i4v d;
@@ -110,21 +143,22 @@ template <int R, int NT, bool TR> struct Stage {
           for (int k = 0; k < 4; ++k) d[k] = v[k][j];
         } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)                    // rows 2k, 2k+1 of the 8 x 4 piece: dwords 4k + j/2 and 4k + 2 + j/2
+          for (int k = 0; k < 4; ++k)                    // dwords j / 2 of rows 2k and 2k + 1
             d[k] = (int)__builtin_amdgcn_perm((unsigned)v[k][2 + j / 2], (unsigned)v[k][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
         }
-        *(i4v*)(lds + swz(cg * 4 + j, c)) = d;
+        *(i4v*)(buf + (lds[j] ^ flip)) = d;
       }
     }
   }
 };
 
-template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>::NT, 2) gemm_kernel(const GemmArgs args) {
-  typedef Cfg<BIG> C;
+template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIND>::NT, 2) gemm_kernel(const GemmArgs) {
+  typedef Cfg<KIND> C;
   constexpr int NT = C::NT, TM = C::TM, TN = C::TN, MI = C::MI, NI = 2;
   constexpr bool TA = FORM == F_TN, TB = FORM != F_NT;
   constexpr bool TWO = EPI == E_GATE2;                   // two accumulators, one after the other
-  __shared__ __attribute__((aligned(16))) char lds[2][(TM + TN) * 128];
+  constexpr uint32_t HALF = (TM + TN) * 128;             // one buffer; a power of two, so that an XOR turns to the other
+  __shared__ __attribute__((aligned(16))) char lds[2 * HALF];
 
   // ---- which tile.  Workgroups go to the 8 dies in turn: die x takes the x-th eighth of the tiles, so that tiles that share rows or columns
   // share an L2; within it, 8 row tiles at a time.
@@ -133,10 +167,13 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
     const uint32_t n = gridDim.x, q = n / 8, r = n % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
     b = (int64_t)x * q + (x < r ? x : r) + i;
   }
+  // (the arguments where they lie, by the scalar unit: indexing the parameter itself would copy it to scratch)
+  const GemmArgs& all = *(const GemmArgs*)__builtin_amdgcn_kernarg_segment_ptr();
   int pi = 0;
-  for (int i = 1; i < args.n; ++i)
-    if (b >= args.p[i].tile0) pi = i;
-  const Prob& P = args.p[pi];
+  if constexpr (FORM == F_TN)
+    for (int i = 1; i < all.n; ++i)
+      if (b >= all.p[i].tile0) pi = i;
+  const Prob& P = all.p[pi];
   b -= P.tile0;
   const int64_t per = P.tm * P.tn;
   const int split = (int)(b / per);
@@ -147,65 +184,29 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
   const int64_t m0 = tmi * TM, n0 = tni * OUTN;
   const int64_t M = P.M, N = P.N;
 
-  Stage<TM, NT, TA> sa;
-  Stage<TN, NT, TB> sb;
-  const int64_t lda0 = P.lda[0], lda1 = P.lda[1], ldb0 = P.ldb[0], ldb1 = P.ldb[1];
-  const int64_t nb0 = P.nb0;
-  int cur = -1;                                          // segment whose row offsets are in sa / sb
-  auto aim = [&](int seg) {
-    const int64_t la = seg ? lda1 : lda0, lb = seg ? ldb1 : ldb0;
-    sa.init([&](int r) { const int64_t left = M - 1 - m0; return (r < left ? r : left) * la; });   // rows behind the last: the last (never stored)
-    if constexpr (EPI == E_GATE) {
-      // rows 64 w .. 64 w + 31 of the tile are the gate's columns of wave column w, the next 32 the other weight's (loaded with its own base)
-      sb.init([&](int r) { const int64_t left = N - 1 - n0; const int col = (r >> 6) * 32 + (r & 31); return (col < left ? col : left) * (r & 32 ? ldb1 : ldb0); });
-    } else {
-      sb.init([&](int r) { const int64_t left = N - 1 - n0; return (r < left ? r : left) * lb; });
-    }
-    cur = seg;
-  };
-  const bool inA = !TA || m0 + TM <= M, inB = !TB || n0 + TN <= N;
-
-  auto fetch = [&](int64_t i) {
-    const int seg = i >= nb0;
-    if (seg != cur) aim(seg);
-    const int64_t k = (i - (seg ? nb0 : 0)) * BK, nk = (seg ? P.K[1] : P.K[0]) - k;
-    const int64_t la = seg ? lda1 : lda0, lb = seg ? ldb1 : ldb0;
-    const T* A = (const T*)(seg ? P.A[1] : P.A[0]);
-    const T* B = (const T*)(seg ? P.B[1] : P.B[0]);
-    if constexpr (TA) {
-      if (nk >= BK && inA) sa.template load_col<false>(A + k * la + m0, la, nk, M - m0);
-      else sa.template load_col<true>(A + k * la + m0, la, nk, M - m0);
-    } else {
-      if (nk >= BK) sa.load_row(A + m0 * la + k);
-      else sa.load_row_guard(A + m0 * la + k, nk);
-    }
-    if constexpr (TB) {
-      if (nk >= BK && inB) sb.template load_col<false>(B + k * lb + n0, lb, nk, N - n0);
-      else sb.template load_col<true>(B + k * lb + n0, lb, nk, N - n0);
-    } else if constexpr (EPI == E_GATE) {
-      // chunk i of a thread is row t / 8 + i * NT / 8; NT / 8 is 32 or 64
-      const T *W0 = B + n0 * ldb0 + k, *W1 = (const T*)P.B[1] + n0 * ldb1 + k;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = ((int)threadIdx.x >> 3) + i * (NT / 8);
-        const T* p = (const T*)((const char*)(r & 32 ? W1 : W0) + sb.off[i]);
-        if (nk >= BK) {
-          sb.v[i] = ld_any<i4v>(p);
-        } else {
-          T t[KE];
-          raw_guard<KE>(p, nk - sb.c * KE, t);
-          sb.v[i] = __builtin_bit_cast(i4v, t);
-        }
-      }
-    } else {
-      if (nk >= BK) sb.load_row(B + n0 * lb + k);
-      else sb.load_row_guard(B + n0 * lb + k, nk);
-    }
-  };
-
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int lr = lane & 31, lh = lane >> 5;
+
+  // ---- operands
+  Stage<TM, NT, TA> sa;
+  Stage<TN, NT, TB> sb;
+  sa.init_lds(0);
+  sb.init_lds(TM * 128);
+  const int64_t lda0 = P.lda[0], lda1 = P.lda[1], ldb0 = P.ldb[0], ldb1 = P.ldb[1];
+  const int64_t nb0 = P.nb0, K0 = P.K[0], K1 = P.K[1];
+  // E_GATE: rows 64 w .. 64 w + 31 of the tile's B are the gate's columns of wave column w, the next 32 the other weight's
+  int other = 0;
+  if constexpr (EPI == E_GATE)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) other |= ((wave * 8 + i * (NT / 8)) >> 5 & 1) << i;
+  // a tile that hangs over the last column of a col operand: its last group of four may read up to three elements into the rows that follow,
+  // which must exist
+  const int spare = (TA && m0 + TM > M) || (TB && n0 + TN > N) ? 4 : 0;
+  const T *pa = nullptr, *pb = nullptr, *pb1 = nullptr;  // the next block's base
+  int64_t la = 0, lb = 0;
+  int64_t run = 0;                                       // blocks from `pa`, `pb` on that need no guard
+  int cur = -1;                                          // segment that the row offsets are for
 
   f16v acc[TWO ? 2 : 1][MI][NI];
 #pragma unroll
@@ -215,51 +216,86 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[a][i][j] = (f16v)(0.f);
 
-  const int64_t ib = P.nb * split / P.splits, ie = P.nb * (split + 1) / P.splits;
-  auto multiply = [&](f16v (&c)[MI][NI], const char* buf) {
-    const char* la = buf + 0;
-    const char* lb = buf + TM * 128;
+  // ---- one block: four steps of two chunks.  Row r + 32 has its chunks at c ^ 4 of row r, so four offsets serve every row of a lane
+  uint32_t oa[4], ob[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    oa[s] = swz(wm * (MI * 32) + lr, 2 * s + lh);
+    ob[s] = TM * 128 + swz(wn * 64 + lr, 2 * s + lh);
+  }
+  auto multiply = [&](f16v (&c)[MI][NI], uint32_t flip) BLK_INLINE {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       i4v fa[MI], fb[NI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = *(const i4v*)(la + swz(wm * (MI * 32) + i * 32 + lr, 2 * s + lh));
+      for (int j = 0; j < NI; ++j) fb[j] = *(const i4v*)(lds + ((ob[s ^ (j & 1 ? 2 : 0)] + j * 4096) ^ flip));
 #pragma unroll
-      for (int j = 0; j < NI; ++j) fb[j] = *(const i4v*)(lb + swz(wn * 64 + j * 32 + lr, 2 * s + lh));
+      for (int i = 0; i < MI; ++i) fa[i] = *(const i4v*)(lds + ((oa[s ^ (i & 1 ? 2 : 0)] + i * 4096) ^ flip));
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) c[i][j] = mfma(fb[j], fa[i], c[i][j]);
     }
   };
-  auto loop = [&](f16v (&c)[MI][NI], int64_t from, int64_t to) {
-    for (int64_t i = from; i < to; ++i) {
-      if (i + 1 < ie) fetch(i + 1);
-      multiply(c, lds[(i - ib) & 1]);
-      if (i + 1 < ie) {
-        char* d = lds[(i + 1 - ib) & 1];
-        sa.store(d);
-        sb.store(d + TM * 128);
+
+  const int64_t ib = P.nb * split / P.splits, ie = P.nb * (split + 1) / P.splits;
+  uint32_t flip = HALF;                                  // the buffer being multiplied
+#pragma unroll
+  for (int h = 0; h < (TWO ? 2 : 1); ++h)
+    for (int64_t i = h ? nb0 : ib - 1; i < (TWO && !h ? nb0 : ie); ++i) {
+      // ---- block i + 1 into registers
+      const bool more = i + 1 < ie;
+      if (more) {
+        int64_t nk = 0;
+        if (run == 0) {                                  // a segment's first block, or one of its last
+          const int seg = i + 1 >= nb0;
+          const int64_t j = i + 1 - (seg ? nb0 : 0), k = j * BK, K = seg ? K1 : K0;
+          if (seg != cur) {
+            cur = seg;
+            la = seg ? lda1 : lda0;
+            lb = seg ? ldb1 : ldb0;
+            // rows behind an operand's last: the last one again, not stored
+            if constexpr (TA) sa.aim_cols(la, M - m0);
+            else sa.aim_rows([&](int r) BLK_INLINE { const int64_t left = M - 1 - m0; return (r < left ? r : left) * la; });
+            if constexpr (TB) sb.aim_cols(lb, N - n0);
+            else if constexpr (EPI == E_GATE)
+              sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; const int c = (r >> 6) * 32 + (r & 31); return (c < left ? c : left) * (r & 32 ? ldb1 : ldb0); });
+            else
+              sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; return (r < left ? r : left) * lb; });
+          }
+          pa = (const T*)(seg ? P.A[1] : P.A[0]) + (TA ? k * la + m0 : m0 * la + k);
+          pb = (const T*)(seg ? P.B[1] : P.B[0]) + (TB ? k * lb + n0 : n0 * lb + k);
+          if constexpr (EPI == E_GATE) pb1 = (const T*)P.B[1] + n0 * ldb1 + k;
+          run = K - spare > 0 ? (K - spare) / BK - j : 0;
+          if (run <= 0) {
+            run = 0;
+            nk = K - k;
+          }
+        }
+        if (run > 0) {
+          sa.load(pa, pa, 0, la);
+          sb.load(pb, pb1, other, lb);
+          pa += TA ? BK * la : BK;
+          pb += TB ? BK * lb : BK;
+          if constexpr (EPI == E_GATE) pb1 += BK;
+          --run;
+        } else {
+          sa.load_guard(pa, pa, 0, la, nk, M - m0);
+          sb.load_guard(pb, pb1, other, lb, nk, N - n0);
+        }
+      }
+      if (h || i >= ib) multiply(acc[TWO ? h : 0], flip);
+      flip ^= HALF;
+      if (more) {
+        sa.store(lds, flip);
+        sb.store(lds, flip);
       }
       __syncthreads();
     }
-  };
-  if (ib < ie) {
-    fetch(ib);
-    sa.store(lds[0]);
-    sb.store(lds[0] + TM * 128);
-  }
-  __syncthreads();
-  if constexpr (TWO) {
-    loop(acc[0], ib, nb0);
-    loop(acc[1], nb0, ie);
-  } else {
-    loop(acc[0], ib, ie);
-  }
 
   // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows
   constexpr int PITCH = 68;                              // floats: 272 bytes, so that 8 rows' 16-byte pieces lie in different banks
-  float* st = (float*)&lds[0][0] + wave * (32 * PITCH);
+  float* st = (float*)lds + wave * (32 * PITCH);
   static_assert(sizeof(lds) >= (size_t)(NT / 64) * 32 * PITCH * 4, "epilogue staging");
   constexpr bool PAIR = EPI == E_GATE || EPI == E_GATE2;
   const int act = P.act;
@@ -302,7 +338,7 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
           } else {
             float g[8], y[8];
             load_n<float, 8>(P.save0 + m * N + n, nv, g);
-            act_d8<FINE>(act, g, y);
+            act_d_n<FINE, 8>(act, g, y);
             if (P.save1) {
               load_n<float, 8>(P.save1 + m * N + n, nv, u);
 #pragma unroll
@@ -326,7 +362,7 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
             for (int e = 0; e < 8; ++e) v[e] += t[e];
           }
           if (P.save0) store_n<float, 8>(P.save0 + m * N + n, nv, v);
-          act8<FINE>(act, v);
+          act_n<FINE, 8>(act, v);
           if constexpr (PAIR) {
             if (P.bias1) {
               load_n<T, 8>((const T*)P.bias1 + n, nv, t);
@@ -350,22 +386,177 @@ template <int FORM, int EPI, int BIG> __global__ void __launch_bounds__(Cfg<BIG>
     }
 }
 
-template <int FORM, int EPI, int BIG> int go(const GemmArgs& a, int64_t tiles, hipStream_t s) {
-  hipLaunchKernelGGL((gemm_kernel<FORM, EPI, BIG>), dim3((unsigned)tiles), dim3(Cfg<BIG>::NT), 0, s, a);
+// ---- few rows (M <= 64): the weights are read once and nothing else counts, so a workgroup takes 16 columns of C and its W waves share the
+// summed index; each lane loads its 16 bytes of a weight row straight into the matrix instruction's operand (16x16, the weight's 16 rows on
+// the first side), a batch of loads at a time.  The waves' sums meet in LDS and are added in the waves' order.
+__device__ __forceinline__ f4 mfma16(i4v a, i4v b, f4 c) {
+  if constexpr (sizeof(T) == 4) {
+    const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+}
+
+template <int MT, int W, int NW> struct Few {
+  static constexpr int KS = 4 * KE, UN = MT == 1 ? 8 : 4;
+  const T* x[MT];
+  const T* w[NW];
+  f4 (*acc)[MT];                                         // [NW][MT]
+
+  // steps s0 .. s0 + UN - 1, of which those from `lim` on count as zeros
+  template <bool ALL> __device__ __forceinline__ void batch(int64_t s0, int64_t lim) {
+    i4v fx[UN][MT], fw[UN][NW];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int64_t k = (ALL || s0 + u < lim ? s0 + u : lim - 1) * KS;
+#pragma unroll
+      for (int j = 0; j < NW; ++j) fw[u][j] = ld_any<i4v>(w[j] + k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fx[u][i] = ld_any<i4v>(x[i] + k);
+    }
+    __builtin_amdgcn_sched_barrier(0);                   // all loads of the batch before the first product
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (!ALL && s0 + u >= lim) break;                  // (uniform)
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = mfma16(fw[u][j], fx[u][i], acc[j][i]);
+    }
+  }
+  __device__ __forceinline__ void run(int64_t K, int wave) {
+    const int lq = (threadIdx.x & 63) >> 4;
+    const int64_t steps = (K + KS - 1) / KS, full = K / KS;
+    const int64_t from = steps * wave / W, to = steps * (wave + 1) / W, lim = to < full ? to : full;
+    int64_t s = from;
+    for (; s + UN <= lim; s += UN) batch<true>(s, lim);
+    if (s < lim) batch<false>(s, lim);
+    if (to > full && to > from) {                        // the last, partial step
+      const int64_t k = full * KS, nk = K - k - lq * KE;
+      T o[KE];
+      i4v fx[MT], fw[NW];
+#pragma unroll
+      for (int j = 0; j < NW; ++j) { raw_guard<KE>(w[j] + k, nk, o); fw[j] = __builtin_bit_cast(i4v, o); }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) { raw_guard<KE>(x[i] + k, nk, o); fx[i] = __builtin_bit_cast(i4v, o); }
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = mfma16(fw[j], fx[i], acc[j][i]);
+    }
+  }
+};
+
+template <int EPI, int MT, int W> __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 16 ? 4 : 2, W == 16 ? 4 : 3))) few_kernel(const GemmArgs args) {
+  constexpr int NA = EPI == E_LIN ? 1 : 2;
+  __shared__ f4 red[W][NA][MT][64];
+  const Prob& P = args.p[0];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
+  const int64_t M = P.M, N = P.N, n0 = (int64_t)blockIdx.x * 16;
+  const int64_t wr = n0 + lr < N ? n0 + lr : N - 1;      // columns behind N, rows behind M: the last again, not stored
+  f4 acc[NA][MT];
+#pragma unroll
+  for (int j = 0; j < NA; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f4{0.f, 0.f, 0.f, 0.f};
+  auto rows = [&](const T* (&x)[MT], int seg) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = i * 16 + lr < M ? i * 16 + lr : M - 1;
+      x[i] = (const T*)P.A[seg] + m * P.lda[seg] + lq * KE;
+    }
+  };
+  const T* w0 = (const T*)P.B[0] + wr * P.ldb[0] + lq * KE;
+  const T* w1 = NA == 2 ? (const T*)P.B[1] + wr * P.ldb[1] + lq * KE : nullptr;
+  if constexpr (EPI == E_GATE) {
+    Few<MT, W, 2> f;
+    rows(f.x, 0);
+    f.w[0] = w0;
+    f.w[1] = w1;
+    f.acc = acc;
+    f.run(P.K[0], wave);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+      Few<MT, W, 1> f;
+      rows(f.x, j);
+      f.w[0] = j ? w1 : w0;
+      f.acc = acc + j;
+      f.run(P.K[j], wave);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NA; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) red[wave][j][i][lane] = acc[j][i];
+  __syncthreads();
+  for (int q = threadIdx.x; q < MT * 64; q += 64 * W) {
+    const int i = q >> 6, l = q & 63;
+    const int64_t m = i * 16 + (l & 15), n = n0 + (l >> 4) * 4;
+    if (m >= M || n >= N) continue;
+    const int nv = N - n < 4 ? (int)(N - n) : 4;
+    float v[NA][4], t[4];
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+      f4 s = red[0][j][i][l];
+#pragma unroll
+      for (int k = 1; k < W; ++k) s += red[k][j][i][l];
+      const T* bias = (const T*)(j ? P.bias1 : P.bias0);
+      if (bias) load_n<T, 4>(bias + n, nv, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = bias ? s[e] + t[e] : s[e];
+      float* save = j ? P.save1 : P.save0;
+      if (save) store_n<float, 4>(save + m * N + n, nv, v[j]);
+    }
+    act_n<FINE, 4>(P.act, v[0]);
+    if constexpr (NA == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[0][e] *= v[1][e];
+    }
+    if (P.addend) {
+      load_n<T, 4>((const T*)P.addend + m * P.ldadd + n, nv, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[0][e] += t[e];
+    }
+    store_n<T, 4>((T*)P.out0 + m * P.ldo + n, nv, v[0]);
+  }
+}
+
+template <int EPI> int few(const GemmArgs& a, int64_t blocks, hipStream_t s) {
+  const Prob& p = a.p[0];
+  const int64_t K = p.K[0] > p.K[1] ? p.K[0] : p.K[1];
+  // 16 waves where 4 would each have more than one batch of eight steps to wait for
+  if (p.M > 16) hipLaunchKernelGGL((few_kernel<EPI, 4, 8>), dim3((unsigned)blocks), dim3(512), 0, s, a);
+  else if (K > 4 * 8 * 4 * KE) hipLaunchKernelGGL((few_kernel<EPI, 1, 16>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((few_kernel<EPI, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  DPVO_LAUNCH_CHECK();
+  return DPVO_OK;
+}
+
+template <int FORM, int EPI, int KIND> int go(const GemmArgs& a, int64_t tiles, hipStream_t s) {
+  hipLaunchKernelGGL((gemm_kernel<FORM, EPI, KIND>), dim3((unsigned)tiles), dim3(Cfg<KIND>::NT), 0, s, a);
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
 
 }  // namespace
 
-int BLK_ENTRY(const GemmArgs& a, int form, int epi, int big, int64_t tiles, hipStream_t s) {
+int BLK_ENTRY(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s) {
   if (tiles == 0) return DPVO_OK;
-  if (form == F_NT && epi == E_LIN) return go<F_NT, E_LIN, 0>(a, tiles, s);
-  if (form == F_NT && epi == E_GATE) return go<F_NT, E_GATE, 0>(a, tiles, s);
-  if (form == F_NT && epi == E_GATE2) return go<F_NT, E_GATE2, 0>(a, tiles, s);
-  if (form == F_NN && epi == E_LIN) return go<F_NN, E_LIN, 0>(a, tiles, s);
-  if (form == F_NN && epi == E_DACT) return go<F_NN, E_DACT, 0>(a, tiles, s);
-  if (form == F_TN && epi == E_LIN) return go<F_TN, E_LIN, 0>(a, tiles, s);
+  if (kind == T_FEW) return epi == E_LIN ? few<E_LIN>(a, tiles, s) : epi == E_GATE ? few<E_GATE>(a, tiles, s) : few<E_GATE2>(a, tiles, s);
+#define BLK_GO(F, E) if (form == F && epi == E) return kind == T_BIG ? go<F, E, T_BIG>(a, tiles, s) : kind == T_SMALL ? go<F, E, T_SMALL>(a, tiles, s) : go<F, E, T_TILE>(a, tiles, s);
+  BLK_GO(F_NT, E_LIN)
+  BLK_GO(F_NT, E_GATE)
+  BLK_GO(F_NN, E_LIN)
+  BLK_GO(F_NN, E_DACT)
+  BLK_GO(F_TN, E_LIN)
+#undef BLK_GO
+  if (form == F_NT && epi == E_GATE2) return kind == T_SMALL ? go<F_NT, E_GATE2, T_SMALL>(a, tiles, s) : go<F_NT, E_GATE2, T_TILE>(a, tiles, s);
   return DPVO_E_UNSUPPORTED;
 }
 

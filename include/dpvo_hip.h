@@ -608,7 +608,7 @@ int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, cons
 /* Input gradient dx [M,N] = a0 b0 [+ a1 b1] [+ addend]: a_s [M,K_s] gradients of the sums, b_s [K_s,N] the weights as stored.
  * With `gate` (f32 [M,N] contiguous, as saved) dx is itself the gradient of act(gate) [* up] and is taken through it at once:
  * dx = d_gate, dx2 = d_up as in dpvo_gated_linear_dact; with `mask` [M,N] (the ReLU's output) dx is kept where mask > 0.
- * addend is allowed with neither.  ws: dpvo_gated_linear_dx_workspace_bytes(M, N, K0 + K1) bytes (0 when few parts are needed). */
+ * addend is allowed with neither.  ws: dpvo_gated_linear_dx_workspace_bytes(p) bytes (0: the sum is not cut into parts). */
 typedef struct {
   const void *a[2], *b[2], *addend, *mask;
   const float *gate, *up;
@@ -617,7 +617,7 @@ typedef struct {
   int64_t M, N;
   int32_t dtype, activation;
 } dpvo_gated_linear_dx_t;
-size_t dpvo_gated_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t dpvo_gated_linear_dx_workspace_bytes(const dpvo_gated_linear_dx_t* p);
 int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, size_t ws_bytes, void* stream);
 
 /* Weight gradients, up to four at once: dw_i [N_i,K_i] = a_i^T b_i over the M rows of a_i [M,N_i] (gradient of a sum) and b_i [M,K_i] (its
