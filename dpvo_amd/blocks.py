@@ -50,6 +50,8 @@ def _check(what, x, *others):
 def _check_layer(what, x, K, w, b, name):
     if w.dim() != 2 or w.shape[1] != K:
         _fail(what, f"{name} is {tuple(w.shape)}, its input has {K} features")
+    if 0 in w.shape:
+        _fail(what, f"{name} is {tuple(w.shape)}: no features")
     if w.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
         _fail(what, f"{name} and its bias must have the input's dtype {x.dtype}")
     if b is not None and tuple(b.shape) != (w.shape[0],):
@@ -180,10 +182,10 @@ def _dw(jobs):
         a, lda = _rows(a)
         b, ldb = _rows(b)
         i = p.n
-        dw = torch.empty(a.shape[1], b.shape[1], dtype=a.dtype, device=a.device) if want_w else None
+        dw = torch.empty(a.shape[1], b.shape[1], dtype=a.dtype, device=a.device)      # (db is made beside it)
         db = torch.empty(a.shape[1], dtype=a.dtype, device=a.device) if want_b else None
-        keep += [a, b]
-        out.append((dw, db))
+        keep += [a, b, dw]
+        out.append((dw if want_w else None, db))
         p.a[i], p.b[i], p.dw[i], p.db[i], p.lda[i], p.ldb[i], p.N[i], p.K[i] = _p(a), _p(b), _p(dw), _p(db), lda, ldb, a.shape[1], b.shape[1]
         p.n = i + 1
     if p.n:

@@ -21,31 +21,45 @@ int gemm(const GemmArgs& a, int dtype, int form, int epi, int kind, int64_t tile
 }
 inline int block_k(int dtype) { return dtype == DPVO_F32 ? 32 : 64; }
 
-// out[e] = sum over splits of part[split][e] (+ addend[e]), all contiguous
-template <class T> __global__ void __launch_bounds__(256) split_sum_kernel(const float* part, int64_t size, int splits, const T* addend, T* out) {
+// out[e] = sum over parts of part[i][e] (+ addend[e]), all contiguous; a job for each row of the grid
+struct SumJob {
+  const float* part;
+  int64_t size;
+  const void* addend;
+  void* out;
+};
+struct SumArgs {
+  SumJob j[2 * MAXP];
+  int n, splits;
+};
+template <class T> __global__ void __launch_bounds__(256) split_sum_kernel(const SumArgs a) {
+  const SumJob& j = ((const SumArgs*)__builtin_amdgcn_kernarg_segment_ptr())->j[blockIdx.y];
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (e >= size) return;
-  const int nv = size - e < 4 ? (int)(size - e) : 4;
+  if (e >= j.size) return;
+  const int nv = j.size - e < 4 ? (int)(j.size - e) : 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f}, t[4];
-  for (int s = 0; s < splits; ++s) {
-    load_n<float, 4>(part + s * size + e, nv, t);
+  for (int s = 0; s < a.splits; ++s) {
+    load_n<float, 4>(j.part + s * j.size + e, nv, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += t[i];
   }
-  if (addend) {
-    load_n<T, 4>(addend + e, nv, t);
+  if (j.addend) {
+    load_n<T, 4>((const T*)j.addend + e, nv, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += t[i];
   }
-  store_n<T, 4>(out + e, nv, v);
+  store_n<T, 4>((T*)j.out + e, nv, v);
 }
-int split_sum(const float* part, int64_t size, int splits, const void* addend, void* out, int dtype, hipStream_t s) {
+int split_sum(const SumArgs& a, int dtype, hipStream_t s) {
+  int64_t size = 0;
+  for (int i = 0; i < a.n; ++i) size = a.j[i].size > size ? a.j[i].size : size;
   if (size == 0) return DPVO_OK;
   const int64_t blocks = cdiv64(cdiv64(size, 4), 256);
   if (blocks > INT_MAX) return DPVO_E_UNSUPPORTED;
-  if (dtype == DPVO_F16) hipLaunchKernelGGL((split_sum_kernel<_Float16>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const _Float16*)addend, (_Float16*)out);
-  else if (dtype == DPVO_BF16) hipLaunchKernelGGL((split_sum_kernel<__bf16>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const __bf16*)addend, (__bf16*)out);
-  else hipLaunchKernelGGL((split_sum_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, part, size, splits, (const float*)addend, (float*)out);
+  const dim3 grid((unsigned)blocks, (unsigned)a.n);
+  if (dtype == DPVO_F16) hipLaunchKernelGGL((split_sum_kernel<_Float16>), grid, dim3(256), 0, s, a);
+  else if (dtype == DPVO_BF16) hipLaunchKernelGGL((split_sum_kernel<__bf16>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((split_sum_kernel<float>), grid, dim3(256), 0, s, a);
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
@@ -73,52 +87,19 @@ template <class T> __global__ void __launch_bounds__(256) dact_kernel(const T* d
   }
 }
 
-// ---- column sums: rows -> partial rows (a workgroup: 256 columns, its share of the rows), partial rows -> one
+// ---- partial rows -> rows
 struct ColJob {
-  const void* a;
   float* part;
   void* out;
-  int64_t lda, M, N;                                     // M rows of N
+  int64_t N;
   int64_t parts;                                         // partial rows to one output row
   int64_t outs;                                          // output rows
-  int type;                                              // of `a` (first pass), of `out` (second)
+  int type;                                              // of `out`
 };
 struct ColArgs {
   ColJob j[5];
   int n;
 };
-template <class T> __device__ __forceinline__ void col_rows(const T* a, int64_t lda, int64_t r0, int64_t r1, int nv, float (&v)[8]) {
-  float t[8];
-  for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += 8) {
-    load_n<T, 8>(a + r * lda, nv, t);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += t[e];
-  }
-}
-__global__ void __launch_bounds__(256) col_sum_kernel(const ColArgs args) {
-  __shared__ float lds[8][256 + 8];
-  const ColJob& j = args.j[blockIdx.z];
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x % 32 * 8;
-  if ((int64_t)blockIdx.x * 256 >= j.N) return;          // (another job's columns; the whole workgroup)
-  const int64_t r0 = j.M * blockIdx.y / gridDim.y, r1 = j.M * (blockIdx.y + 1) / gridDim.y;
-  float v[8] = {};
-  if (n < j.N) {
-    const int nv = j.N - n < 8 ? (int)(j.N - n) : 8;
-    if (j.type == DPVO_F16) col_rows((const _Float16*)j.a + n, j.lda, r0, r1, nv, v);
-    else if (j.type == DPVO_BF16) col_rows((const __bf16*)j.a + n, j.lda, r0, r1, nv, v);
-    else col_rows((const float*)j.a + n, j.lda, r0, r1, nv, v);
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) lds[threadIdx.x / 32][threadIdx.x % 32 * 8 + e] = v[e];
-  __syncthreads();
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c < j.N) {
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s += lds[k][threadIdx.x];
-    j.part[blockIdx.y * j.N + c] = s;
-  }
-}
 // out[o][c] = sum of part[o * parts + p][c]: 64 columns x 4 shares of the partial rows
 __global__ void __launch_bounds__(256) col_reduce_kernel(const ColArgs args) {
   __shared__ float lds[4][64];
@@ -152,8 +133,6 @@ int col_reduce(const ColArgs& c, hipStream_t s) {
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
-int64_t col_parts(int64_t M) { return M < 64 ? 1 : M / 64 < 256 ? M / 64 : 256; }
-
 // ---- which tiles, and in how many parts the summed index is cut where there are too few of them
 struct Plan {
   int kind;
@@ -169,13 +148,17 @@ template <class F> Plan plan(F count, int64_t nb, int dtype, bool cut) {
   if (dtype != DPVO_F32 && nb >= 12 && count(256) >= 200) return {T_BIG, 1};
   const int64_t t = count(128);
   if (t >= 384) return {T_TILE, 1};
-  if (cut && t > 0) {
-    int64_t s = 512 / t;
-    if (s > nb / 8) s = nb / 8;
-    if (s > 64) s = 64;
-    if (s > 1) return {T_TILE, s};
-  }
-  return {T_SMALL, 1};
+  if (!cut || t == 0) return {T_SMALL, 1};
+  // parts: towards two workgroups on each of 256 compute units, each with 8 blocks at least (a part costs a tile's write and read in f32);
+  // where that does not even give one each, small tiles with 4 blocks at least.  dw 384 x 384 over 45312 rows: 45 us in 56 parts, 56 in 64 and
+  // 59 in 16; over 9216: 23 us with small tiles in 21, 25 with large ones in 16.
+  auto parts = [&](int64_t want, int64_t least) {
+    const int64_t n = want < nb / least ? want : nb / least;
+    return n < 1 ? 1 : n > 64 ? 64 : n;
+  };
+  const int64_t n = parts(512 / t, 8);
+  if (n * t >= 256) return {T_TILE, n};
+  return {T_SMALL, parts(768 / count(64), 4)};
 }
 inline int64_t tiles(int64_t M, int64_t N, int t) { return cdiv64(M, t) * cdiv64(N, t); }
 int64_t tiles_of(Prob& p, int kind, int halves = 1) {
@@ -324,18 +307,22 @@ extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, s
     q.splits = (int)c.splits;
     q.part = (float*)ws;
     const int rc = gemm(a, p->dtype, F_NN, E_LIN, c.kind, q.tm * q.tn * c.splits, s);
-    return rc ? rc : split_sum(q.part, p->M * p->N, q.splits, p->addend, p->dx, p->dtype, s);
+    SumArgs sum = {};
+    sum.n = 1;
+    sum.splits = q.splits;
+    sum.j[0] = {q.part, p->M * p->N, p->addend, p->dx};
+    return rc ? rc : split_sum(sum, p->dtype, s);
   }
   q.addend = p->addend; q.ldadd = p->ldadd;
   return gemm(a, p->dtype, F_NN, E_LIN, c.kind, q.tm * q.tn, s);
 }
 
-// workspace: the parts of each product that is split, then the partial column sums
+// workspace: the parts of each product and of its column sums
 static Plan dw_plan(const dpvo_gated_linear_dw_t* p) {
   return plan([&](int t) {
     int64_t n = 0;
     for (int i = 0; i < p->n; ++i)
-      if (p->dw[i]) n += tiles(p->N[i], p->K[i], t);
+      n += tiles(p->N[i], p->K[i], t);
     return n;
   }, cdiv64(p->M, block_k(p->dtype)), p->dtype, true);
 }
@@ -343,9 +330,11 @@ static bool dw_ok(const dpvo_gated_linear_dw_t* p) {
   if (!p || p->n < 0 || p->n > MAXP || !type_ok(p->dtype) || p->M < 0) return false;
   for (int i = 0; i < p->n; ++i) {
     if (p->N[i] < 0 || p->K[i] < 0) return false;
-    if (!p->M || !p->N[i]) continue;
+    if (!p->N[i]) continue;
+    if (p->K[i] ? !p->dw[i] : p->db[i] != nullptr) return false;
+    if (!p->M) continue;
     if (!p->a[i] || !ld_ok(p->lda[i], p->N[i], type_size(p->dtype))) return false;
-    if (p->dw[i] && p->K[i] && (!p->b[i] || !ld_ok(p->ldb[i], p->K[i], type_size(p->dtype)))) return false;
+    if (p->K[i] && (!p->b[i] || !ld_ok(p->ldb[i], p->K[i], type_size(p->dtype)))) return false;
   }
   return true;
 }
@@ -354,8 +343,7 @@ extern "C" size_t dpvo_gated_linear_dw_workspace_bytes(const dpvo_gated_linear_d
   const int64_t s = dw_plan(p).splits;
   int64_t f = 0;
   for (int i = 0; i < p->n; ++i) {
-    if (p->dw[i] && s > 1) f += s * p->N[i] * p->K[i];
-    if (p->db[i]) f += col_parts(p->M) * p->N[i];
+    if (s > 1) f += s * p->N[i] * (p->K[i] + (p->db[i] != nullptr));
   }
   return (size_t)f * 4;
 }
@@ -368,41 +356,30 @@ extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, s
   float* w = (float*)ws;
   GemmArgs a = {};
   int64_t n = 0;
-  int which[MAXP];
+  SumArgs sum = {};
+  sum.splits = (int)splits;
   for (int i = 0; i < p->n; ++i) {
-    if (!p->dw[i] || !p->N[i] || !p->K[i]) continue;
-    Prob& q = a.p[a.n];
-    which[a.n++] = i;
+    if (!p->N[i] || !p->K[i]) continue;
+    Prob& q = a.p[a.n++];
     q.A[0] = p->a[i]; q.B[0] = p->b[i]; q.lda[0] = p->lda[i]; q.ldb[0] = p->ldb[i]; q.K[0] = p->M;
     q.M = p->N[i]; q.N = p->K[i];
     q.nb0 = q.nb = cdiv64(p->M, block_k(p->dtype));
     q.splits = (int)splits;
-    q.out0 = p->dw[i]; q.ldo = p->K[i];
+    q.out0 = p->dw[i]; q.ldo = p->K[i]; q.colsum = p->db[i];
     if (splits > 1) {
-      q.part = w;
+      sum.j[sum.n++] = {q.part = w, q.M * q.N, nullptr, p->dw[i]};
       w += splits * q.M * q.N;
+      if (p->db[i]) {
+        sum.j[sum.n++] = {w, q.M, nullptr, p->db[i]};
+        q.colsum = w;
+        w += splits * q.M;
+      }
     }
     q.tile0 = n;
     n += tiles_of(q, c0.kind) * splits;
   }
-  int rc = gemm(a, p->dtype, F_TN, E_LIN, c0.kind, n, s);
-  if (rc) return rc;
-  if (splits > 1)
-    for (int i = 0; i < a.n; ++i)
-      if ((rc = split_sum(a.p[i].part, a.p[i].M * a.p[i].N, (int)splits, nullptr, p->dw[which[i]], p->dtype, s))) return rc;
-  ColArgs c = {};
-  int64_t width = 0;
-  for (int i = 0; i < p->n; ++i) {
-    if (!p->db[i] || !p->N[i]) continue;
-    ColJob& j = c.j[c.n++];
-    j.a = p->a[i]; j.lda = p->lda[i]; j.M = p->M; j.N = p->N[i]; j.part = w; j.out = p->db[i]; j.parts = col_parts(p->M); j.outs = 1; j.type = p->dtype;
-    w += j.parts * j.N;
-    width = j.N > width ? j.N : width;
-  }
-  if (c.n == 0) return DPVO_OK;
-  hipLaunchKernelGGL(col_sum_kernel, dim3((unsigned)cdiv64(width, 256), (unsigned)col_parts(p->M), (unsigned)c.n), dim3(256), 0, s, c);
-  DPVO_LAUNCH_CHECK();
-  return col_reduce(c, s);
+  const int rc = gemm(a, p->dtype, F_TN, E_LIN, c0.kind, n, s);
+  return rc || splits == 1 ? rc : split_sum(sum, p->dtype, s);
 }
 
 extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {

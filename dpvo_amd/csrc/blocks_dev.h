@@ -125,6 +125,7 @@ struct Prob {
   int64_t M, N;
   const void *bias0, *bias1, *addend, *mask;
   void *out0, *out1;
+  void* colsum;                                          // F_TN: sums of A's columns [M], or with `part` their parts in f32
   float *save0, *save1, *part;
   int64_t ldadd, ldmask, ldo;
   int64_t tile0;                                         // first workgroup of this problem

@@ -130,6 +130,15 @@ template <int R, int NT, bool TR> struct Stage {
       __builtin_memcpy(v, o, sizeof(v));
     }
   }
+  // adds this thread's share of the columns' sums
+  __device__ __forceinline__ void add_cols(float (&sum)[4]) const {
+    T o[KE][4];
+    __builtin_memcpy(o, v, sizeof(o));
+#pragma unroll
+    for (int k = 0; k < KE; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += (float)o[k][j];
+  }
   __device__ __forceinline__ void store(char* buf, uint32_t flip) const {
     if constexpr (!TR) {
 #pragma unroll
@@ -240,6 +249,8 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
 
   const int64_t ib = P.nb * split / P.splits, ie = P.nb * (split + 1) / P.splits;
   uint32_t flip = HALF;                                  // the buffer being multiplied
+  const bool colsum = FORM == F_TN && P.colsum && tni == 0;
+  float cs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int h = 0; h < (TWO ? 2 : 1); ++h)
     for (int64_t i = h ? nb0 : ib - 1; i < (TWO && !h ? nb0 : ie); ++i) {
@@ -287,11 +298,32 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
       if (h || i >= ib) multiply(acc[TWO ? h : 0], flip);
       flip ^= HALF;
       if (more) {
+        if constexpr (FORM == F_TN)
+          if (colsum) sa.add_cols(cs);
         sa.store(lds, flip);
         sb.store(lds, flip);
       }
       __syncthreads();
     }
+
+  // ---- column sums of A (a bias's gradient: the values are in hand, one column of tiles adds them up)
+  if constexpr (FORM == F_TN) {
+    if (colsum) {
+      float* f = (float*)lds;                            // [8][TM]
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[sa.chunk() * TM + sa.col() + j] = cs[j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < TM; c += NT)
+        if (m0 + c < M) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v += f[k * TM + c];
+          if (P.part) ((float*)P.colsum)[split * M + m0 + c] = v;
+          else ((T*)P.colsum)[m0 + c] = (T)v;
+        }
+      __syncthreads();
+    }
+  }
 
   // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows
   constexpr int PITCH = 68;                              // floats: 272 bytes, so that 8 rows' 16-byte pieces lie in different banks

@@ -621,7 +621,7 @@ size_t dpvo_gated_linear_dx_workspace_bytes(const dpvo_gated_linear_dx_t* p);
 int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, size_t ws_bytes, void* stream);
 
 /* Weight gradients, up to four at once: dw_i [N_i,K_i] = a_i^T b_i over the M rows of a_i [M,N_i] (gradient of a sum) and b_i [M,K_i] (its
- * input); db_i [N_i] = column sums of a_i (or NULL).  dw_i contiguous; dw_i == NULL: only db_i. */
+ * input); db_i [N_i] = column sums of a_i, or NULL.  dw_i contiguous. */
 typedef struct {
   const void *a[4], *b[4];
   void *dw[4], *db[4];
