@@ -20,6 +20,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "sigmoid": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
+GATE_ACTIVATIONS = {k: ACTIVATIONS[k] for k in ("identity", "relu", "sigmoid", "silu")}
 NORMS = {None: 0, "layer": 1, "rms": 2}
 MAX_NORM_WIDTH = 16384
 _DTYPES = {torch.float16: L.F16, torch.float32: L.F32, torch.bfloat16: L.BF16}
@@ -90,19 +91,20 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """the current device is the tensors'"""
-
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index is not None and device.index != torch.cuda.current_device() else None
-
+class _Here:
     def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+        pass
 
     def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        pass
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """context: the current device is the tensors'"""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _scratch(nbytes, device):
@@ -131,7 +133,9 @@ def _forward(x, wg, bg, act, v=None, wu=None, bu=None, residual=None, save=False
     su = torch.empty(M, N, dtype=torch.float32, device=x.device) if save and wu is not None else None
     p = L.GatedLinear(_p(x), _p(v) if wu is not None else None, _p(wg), _p(wu), _p(bg), _p(bu), _p(residual), _p(y), _p(sg), _p(su), ldx, ldv,
                       ldwg, ldwu, ldr, N, M, N, x.shape[1], Kv, _DTYPES[x.dtype], act)
-    L.check(L.lib().dpvo_gated_linear(ctypes.byref(p), L.stream()), "dpvo_gated_linear")
+    rc = L.lib().dpvo_gated_linear(ctypes.byref(p), L.stream())
+    if rc:
+        L.check(rc, "dpvo_gated_linear")
     return y, sg, su
 
 
@@ -197,6 +201,11 @@ def _dw(jobs):
     return out
 
 
+def _like(y, x, n):
+    """rows y [M, n] in the leading shape of x"""
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -213,7 +222,7 @@ class _Linear(torch.autograd.Function):
             y, pre, _ = _forward(x, w, b, act, save=act != 0)
         ctx.save_for_backward(x, w, pre)
         ctx.act, ctx.shape = act, x.shape
-        return y.view(*x.shape[:-1], w.shape[0])
+        return _like(y, x, w.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -239,7 +248,7 @@ def linear(x, weight, bias=None, activation="identity"):
     if _wants_grad(x, weight, bias):
         return _Linear.apply(x, weight, bias, act)
     with _on(x.device):
-        return _forward(x, weight, bias, act)[0].view(*x.shape[:-1], weight.shape[0])
+        return _like(_forward(x, weight, bias, act)[0], x, weight.shape[0])
 
 
 # ------------------------------------------------------------------------------------------------------------------ gated linear
@@ -250,7 +259,7 @@ class _GatedLinear(torch.autograd.Function):
             y, g, u = _forward(x, wg, bg, act, v, wu, bu, residual, save=True)
         ctx.save_for_backward(x, v, wg, wu, g, u)
         ctx.act = act
-        return y.view(*x.shape[:-1], wg.shape[0])
+        return _like(y, x, wg.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -292,7 +301,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu", up_
     if _wants_grad(x, w_gate, w_up, b_gate, b_up, up_input, residual):
         return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, up_input, residual, act)
     with _on(x.device):
-        return _forward(x, w_gate, b_gate, act, up_input, w_up, b_up, residual)[0].view(*x.shape[:-1], w_gate.shape[0])
+        return _like(_forward(x, w_gate, b_gate, act, up_input, w_up, b_up, residual)[0], x, w_gate.shape[0])
 
 
 # ------------------------------------------------------------------------------------------------------------------ feed-forward block
@@ -304,7 +313,7 @@ class _FeedForward(torch.autograd.Function):
             y = _forward(h, wd, bd, 0)[0]
         ctx.save_for_backward(x, wg, wu, wd, h, g, u)
         ctx.act = act
-        return y.view(*x.shape[:-1], wd.shape[0])
+        return _like(y, x, wd.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -344,7 +353,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
         return _FeedForward.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     with _on(x.device):
         h = _forward(x, w_gate, b_gate, act, None, w_up, b_up)[0]
-        return _forward(h, w_down, b_down, 0)[0].view(*x.shape[:-1], w_down.shape[0])
+        return _like(_forward(h, w_down, b_down, 0)[0], x, w_down.shape[0])
 
 
 # ------------------------------------------------------------------------------------------------------------------ gated residual block
@@ -399,39 +408,45 @@ def gated_residual(x, w_gate, b_gate, w_in, b_in, w_out, b_out):
         return _GatedResidual.apply(x, w_gate, b_gate, w_in, b_in, w_out, b_out)
     with _on(x.device):
         t = _forward(x, w_in, b_in, _RELU)[0]
-        return _forward(x, w_gate, b_gate, _SIGMOID, t, w_out, b_out, residual=x)[0].view(x.shape)
+        return _like(_forward(x, w_gate, b_gate, _SIGMOID, t, w_out, b_out, residual=x)[0], x, D)
 
 
 # ------------------------------------------------------------------------------------------------------------------ norms
-def _norm_args(x, f, gate, w, b, pw, pb, cfg):
-    """the C struct's inputs, and what must stay alive"""
+def _norm_struct(x, f, gate, w, b, pw, pb, cfg, s, h, ds, dh, grads):
+    """the C struct and what must stay alive (positional: assigning its fields one by one takes longer than the launch)"""
     norm_k, post_k, gate_act, scale, eps, post_eps, h_dtype, groups = cfg
-    p = L.ResidualNorm()
-    x, p.ldx = _rows(x)
-    D = x.shape[1]
+    x, ldx = _rows(x)
+    ldf = ldg = ldds = lddh = 0
     if f is not None:
-        f, p.ldf = _rows(f)
+        f, ldf = _rows(f)
     if gate is not None:
-        gate, p.ldgate = _rows(gate)
-    w, b, pw, pb = (_vector(t) for t in (w, b, pw, pb))
-    p.x, p.f, p.gate, p.w, p.b, p.pw, p.pb = _p(x), _p(f), _p(gate), _p(w), _p(b), _p(pw), _p(pb)
-    p.M, p.D, p.groups = x.shape[0], D, groups
-    p.x_dtype, p.h_dtype = _DTYPES[x.dtype], _DTYPES[h_dtype]
-    p.f_dtype = _DTYPES[f.dtype] if f is not None else p.h_dtype
-    p.w_dtype = next((_DTYPES[t.dtype] for t in (w, b, pw, pb) if t is not None), L.F32)
-    p.norm, p.post, p.gate_activation, p.scale, p.eps, p.post_eps = norm_k, post_k, gate_act, scale, eps, post_eps
-    return p, x, (f, gate, w, b, pw, pb)
+        gate, ldg = _rows(gate)
+    if ds is not None:
+        ds, ldds = _rows(ds)
+    if dh is not None:
+        dh, lddh = _rows(dh)
+    w, b, pw, pb = _vector(w), _vector(b), _vector(pw), _vector(pb)
+    hd = _DTYPES[h_dtype]
+    par = w if w is not None else b if b is not None else pw if pw is not None else pb
+    M, D = x.shape
+    p = L.ResidualNorm(x.data_ptr(), _p(f), _p(gate), _p(w), _p(b), _p(pw), _p(pb), _p(s), _p(h), _p(ds), _p(dh), *map(_p, grads), ldx, ldf, ldg,
+                       ldds, lddh, M, groups, D, _DTYPES[x.dtype], hd if f is None else _DTYPES[f.dtype], hd,
+                       L.F32 if par is None else _DTYPES[par.dtype], norm_k, post_k, gate_act, scale, eps, post_eps)
+    return p, (x, f, gate, w, b, pw, pb, ds, dh)
+
+
+_NO_GRADS = (None,) * 7
 
 
 def _norm_forward(x, f, gate, w, b, pw, pb, cfg):
     """-> s (None without a branch), h (None without a norm)"""
-    shape = x.shape
     with _on(x.device):
-        p, x, keep = _norm_args(x, f, gate, w, b, pw, pb, cfg)
-        s = torch.empty(shape, dtype=x.dtype, device=x.device) if f is not None else None
-        h = torch.empty(shape, dtype=cfg[6], device=x.device) if cfg[0] else None
-        p.s, p.h = _p(s), _p(h)
-        L.check(L.lib().dpvo_residual_norm(ctypes.byref(p), L.stream()), "dpvo_residual_norm")
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
+        h = torch.empty(x.shape, dtype=cfg[6], device=x.device) if cfg[0] else None
+        p, keep = _norm_struct(x, f, gate, w, b, pw, pb, cfg, s, h, None, None, _NO_GRADS)
+        rc = L.lib().dpvo_residual_norm(ctypes.byref(p), L.stream())
+    if rc:
+        L.check(rc, "dpvo_residual_norm")
     return s, h
 
 
@@ -457,13 +472,7 @@ class _ResidualNorm(torch.autograd.Function):
                 if t is not None and ctx.needs_input_grad[i]:
                     grads[i] = make(t.shape, dtype=t.dtype, device=t.device)
             if x.numel():
-                p, _, keep = _norm_args(x, f, gate, w, b, pw, pb, ctx.cfg)
-                if ds is not None:
-                    ds, p.ldds = _rows(ds)
-                if dh is not None:
-                    dh, p.lddh = _rows(dh)
-                p.ds, p.dh = _p(ds), _p(dh)
-                p.dx, p.df, p.dgate, p.dw, p.db, p.dpw, p.dpb = map(_p, grads)
+                p, keep = _norm_struct(x, f, gate, w, b, pw, pb, ctx.cfg, None, None, ds, dh, grads)
                 lib = L.lib()
                 n = lib.dpvo_residual_norm_backward_workspace_bytes(ctypes.byref(p))
                 ws = _scratch(n, x.device)
@@ -536,7 +545,8 @@ def residual_norm(x, branch, weight=None, bias=None, *, norm="layer", eps=1e-3, 
     """s = x + scale * act(gate) * post_norm(branch) and h = norm(s), in one pass: what follows a block and precedes the next.
 
     x, branch [..., D]: of one dtype, or x float32 beside a 16-bit branch.  gate (branch's dtype): shaped like x, or with ones (or nothing) in
-    the place of x's last leading dimensions -- [B, 1, D] gates each of B sequences, [D] everything.  norm, post_norm: "layer", "rms" or None.
+    the place of x's last leading dimensions -- [B, 1, D] gates each of B sequences, [D] everything; gate_activation: "identity", "relu",
+    "sigmoid" or "silu".  norm, post_norm: "layer", "rms" or None.
     -> (s in x's dtype, h in out_dtype: branch's or x's; None if norm is None).  The norm reads s before it is rounded."""
     what = "residual_norm"
     _check(what, x, branch, gate, weight, bias, post_weight, post_bias)
@@ -548,7 +558,7 @@ def residual_norm(x, branch, weight=None, bias=None, *, norm="layer", eps=1e-3, 
         if gate.dtype != branch.dtype:
             _fail(what, f"gate is {gate.dtype}, branch {branch.dtype}")
         rows = _gate_rows(what, x, gate)
-    cfg = (_code(NORMS, norm, what, "norm"), _code(NORMS, post_norm, what, "post_norm"), _code(ACTIVATIONS, gate_activation, what, "gate_activation"),
+    cfg = (_code(NORMS, norm, what, "norm"), _code(NORMS, post_norm, what, "post_norm"), _code(GATE_ACTIVATIONS, gate_activation, what, "gate_activation"),
            float(scale), float(eps), float(eps if post_eps is None else post_eps), _h_dtype(what, x, branch.dtype, out_dtype), rows)
     if norm is None and (weight is not None or bias is not None):
         _fail(what, "weight or bias without a norm")

@@ -76,7 +76,7 @@ template <class T> __global__ void __launch_bounds__(256) dact_kernel(const T* d
     load_n<float, 8>(gate + m * N + n, nv, g);
     if (up) load_n<float, 8>(up + m * N + n, nv, u);
     float o[8];
-    act_d_n<sizeof(T) == 4>(act, g, o);
+    act_d_n<sizeof(T) == 4, true>(act, g, o);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       o[e] *= d[e];
@@ -100,20 +100,33 @@ struct ColArgs {
   ColJob j[5];
   int n;
 };
-// out[o][c] = sum of part[o * parts + p][c]: 64 columns x 4 shares of the partial rows
-__global__ void __launch_bounds__(256) col_reduce_kernel(const ColArgs args) {
-  __shared__ float lds[4][64];
-  const ColJob& j = args.j[blockIdx.z];
+// out[o][c] = sum of part[o * parts + p][c]: 64 columns x 16 shares of the partial rows, eight loads of each under way
+__global__ void __launch_bounds__(1024) col_reduce_kernel(const ColArgs) {
+  __shared__ float lds[16][64];
+  const ColJob& j = ((const ColArgs*)__builtin_amdgcn_kernarg_segment_ptr())->j[blockIdx.z];
   const int64_t c0 = (int64_t)blockIdx.x * 64, c = c0 + threadIdx.x % 64;
+  const int share = threadIdx.x / 64;
   if (c0 >= j.N) return;
   for (int64_t o = blockIdx.y; o < j.outs; o += gridDim.y) {
     float s = 0.f;
-    if (c < j.N)
-      for (int64_t p = threadIdx.x / 64; p < j.parts; p += 4) s += j.part[(o * j.parts + p) * j.N + c];
-    lds[threadIdx.x / 64][threadIdx.x % 64] = s;
+    if (c < j.N) {
+      const float* q = j.part + o * j.parts * j.N + c;
+      int64_t p = share;
+      for (; p + 7 * 16 < j.parts; p += 8 * 16) {
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = q[(p + k * 16) * j.N];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += t[k];
+      }
+      for (; p < j.parts; p += 16) s += q[p * j.N];
+    }
+    lds[share][threadIdx.x % 64] = s;
     __syncthreads();
     if (threadIdx.x < 64 && c < j.N) {
-      s = ((lds[0][threadIdx.x] + lds[1][threadIdx.x]) + lds[2][threadIdx.x]) + lds[3][threadIdx.x];
+      s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s += lds[k][threadIdx.x];
       if (j.type == DPVO_F16) ((_Float16*)j.out)[o * j.N + c] = (_Float16)s;
       else if (j.type == DPVO_BF16) ((__bf16*)j.out)[o * j.N + c] = (__bf16)s;
       else ((float*)j.out)[o * j.N + c] = s;
@@ -129,7 +142,7 @@ int col_reduce(const ColArgs& c, hipStream_t s) {
     o = c.j[i].outs > o ? c.j[i].outs : o;
   }
   if (w == 0 || o == 0) return DPVO_OK;
-  hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)cdiv64(w, 64), (unsigned)(o < 1024 ? o : 1024), (unsigned)c.n), dim3(256), 0, s, c);
+  hipLaunchKernelGGL(col_reduce_kernel, dim3((unsigned)cdiv64(w, 64), (unsigned)(o < 1024 ? o : 1024), (unsigned)c.n), dim3(1024), 0, s, c);
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
@@ -170,24 +183,25 @@ int64_t tiles_of(Prob& p, int kind, int halves = 1) {
 
 // ---- the norm backward's share of rows
 struct NormPlan {
-  NormShape sh;
+  int sh;
   int64_t groups, rpg, gpb, bpg, blocks;
-  bool shared;                                           // the gate's gradient is summed over rows
+  bool shared;                                           // gate rows that several rows share
 };
 NormPlan norm_plan(const dpvo_residual_norm_t& p) {
   NormPlan n;
   n.sh = norm_shape(p.D);
-  n.shared = p.f && p.gate && p.dgate && p.groups < p.M;
+  n.shared = p.f && p.gate && p.groups < p.M;
   n.groups = n.shared ? p.groups : 1;
   n.rpg = n.groups ? p.M / n.groups : 0;
-  // 512 workgroups: enough loads in flight for the memory, few enough that their partial rows stay a few per cent of the traffic
-  const int64_t want = 512, rounds = cdiv64(n.rpg, norm_slots(n.sh));
+  // 4096 waves, four to a SIMD: enough loads in flight for the memory, few enough that their partial rows stay a few per cent of the traffic
+  const int L = NORM_SHAPES[n.sh].L;
+  const int64_t want = L > 64 ? 4096 / (L / 64) : 1024, rounds = cdiv64(n.rpg, norm_slots(n.sh));
   if (n.groups >= want) {
     n.bpg = 1;
     n.gpb = cdiv64(n.groups, want);
   } else {
     n.gpb = 1;
-    n.bpg = want / n.groups;
+    n.bpg = n.groups ? want / n.groups : 1;
     if (n.bpg > rounds) n.bpg = rounds < 1 ? 1 : rounds;
   }
   n.blocks = cdiv64(n.groups, n.gpb) * n.bpg;
@@ -199,12 +213,13 @@ int norm_check(const dpvo_residual_norm_t* p) {
   if (p->h_dtype != p->x_dtype && p->h_dtype != p->f_dtype) return DPVO_E_UNSUPPORTED;
   if (p->norm < DPVO_NORM_NONE || p->norm > DPVO_NORM_RMS || p->post < DPVO_NORM_NONE || p->post > DPVO_NORM_RMS) return DPVO_E_INVALID;
   if (!act_ok(p->gate_activation)) return DPVO_E_INVALID;
-  if (p->D > NORM_MAX_D) return DPVO_E_UNSUPPORTED;
+  if (p->gate_activation > DPVO_ACT_SILU) return DPVO_E_UNSUPPORTED;
+  if (p->D > NORM_MAX_D || p->M > INT_MAX) return DPVO_E_UNSUPPORTED;
   if (p->gate && (p->groups < 1 || p->M % p->groups || !p->f)) return DPVO_E_INVALID;
   if (p->M && !p->x) return DPVO_E_INVALID;
   return DPVO_OK;
 }
-int norm_run(const NormArgs& a, const NormShape& sh, bool back, int64_t blocks, hipStream_t s) {
+int norm_run(const NormArgs& a, int sh, bool back, int64_t blocks, hipStream_t s) {
   if (a.p.f_dtype == DPVO_F16) return norm_f16(a, sh, back, blocks, s);
   if (a.p.f_dtype == DPVO_BF16) return norm_bf16(a, sh, back, blocks, s);
   return norm_f32(a, sh, back, blocks, s);
@@ -389,8 +404,8 @@ extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {
   if (p->ldx < p->D || (p->f && p->ldf < p->D) || (p->gate && p->ldgate < p->D) || (p->norm && !p->h) || (!p->norm && !p->s)) return DPVO_E_INVALID;
   NormArgs a = {};
   a.p = *p;
-  a.rows_per_gate = p->gate ? p->M / p->groups : 1;
-  const NormShape sh = norm_shape(p->D);
+  a.rows_per_gate = p->gate ? (uint32_t)(p->M / p->groups) : 1;
+  const int sh = norm_shape(p->D);
   const int64_t want = cdiv64(p->M, norm_slots(sh));
   return norm_run(a, sh, false, want < 8192 ? want : 8192, (hipStream_t)stream);
 }
@@ -398,7 +413,7 @@ extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {
 extern "C" size_t dpvo_residual_norm_backward_workspace_bytes(const dpvo_residual_norm_t* p) {
   if (norm_check(p) || p->M == 0) return 0;
   const NormPlan n = norm_plan(*p);
-  const int64_t rows = (n.shared ? n.groups * n.bpg : 0) + n.blocks * ((p->dw != nullptr) + (p->db != nullptr) + (p->dpw != nullptr) + (p->dpb != nullptr));
+  const int64_t rows = (n.shared && p->dgate ? n.groups * n.bpg : 0) + n.blocks * ((p->dw != nullptr) + (p->db != nullptr) + (p->dpw != nullptr) + (p->dpb != nullptr));
   return (size_t)(rows * p->D * 4);
 }
 extern "C" int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* ws, size_t ws_bytes, void* stream) {
@@ -413,7 +428,7 @@ extern "C" int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* 
   ColArgs c = {};
   float* w = (float*)ws;
   const NormPlan n = p->M ? norm_plan(*p) : NormPlan{norm_shape(p->D), 0, 0, 1, 1, 0, false};
-  a.rows_per_gate = p->gate && p->M ? p->M / p->groups : 1;
+  a.shared = n.shared;
   a.groups = n.groups; a.rpg = n.rpg; a.gpb = n.gpb; a.bpg = n.bpg;
   auto job = [&](void* out, int type, int64_t outs, int64_t parts) {
     if (!out) return (float*)nullptr;

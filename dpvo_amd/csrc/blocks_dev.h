@@ -3,6 +3,8 @@
 #pragma once
 #include "common.h"
 
+#define BLK_INLINE __attribute__((always_inline))      // for lambdas: one that stays a call keeps its captures in scratch
+
 namespace blk {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -46,20 +48,21 @@ template <class T, int N> __device__ __forceinline__ void store_n(T* p, int nv, 
   }
 }
 
-// ---- activations.  FINE: expf / tanhf (f32 operands); otherwise the hardware exponential, whose error (a few 2^-22) is far below the half
-// step of a 16-bit result (2^-11 / 2^-8).
+// ---- activations.  FINE: expf / tanhf / division (f32 operands); otherwise the hardware exponential and reciprocal, whose error (a few
+// 2^-22) is far below the half step of a 16-bit result (2^-11 / 2^-8).
 template <bool FINE> __device__ __forceinline__ float exp_(float x) { return FINE ? expf(x) : __expf(x); }
-template <bool FINE> __device__ __forceinline__ float sigmoid_(float x) { return 1.f / (1.f + exp_<FINE>(-x)); }
+template <bool FINE> __device__ __forceinline__ float rcp_(float x) { return FINE ? 1.f / x : __builtin_amdgcn_rcpf(x); }
+template <bool FINE> __device__ __forceinline__ float sigmoid_(float x) { return rcp_<FINE>(1.f + exp_<FINE>(-x)); }
 template <bool FINE> __device__ __forceinline__ float tanh_(float x) {
   if constexpr (FINE) return tanhf(x);
-  return 1.f - 2.f / (1.f + __expf(2.f * x));          // x -> +-inf: exp -> inf / 0, result -> +-1
+  return 1.f - 2.f * rcp_<FINE>(1.f + __expf(2.f * x));  // x -> +-inf: exp -> inf / 0, result -> +-1
 }
 
 template <bool FINE> __device__ __forceinline__ float act_(int a, float z) {
   switch (a) {
     case DPVO_ACT_RELU: return z < 0.f ? 0.f : z;                                    // (NaN stays NaN)
     case DPVO_ACT_SIGMOID: return sigmoid_<FINE>(z);
-    case DPVO_ACT_SILU: return z / (1.f + exp_<FINE>(-z));
+    case DPVO_ACT_SILU: return FINE ? z / (1.f + exp_<FINE>(-z)) : z * sigmoid_<FINE>(z);
     case DPVO_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     case DPVO_ACT_GELU_TANH: return 0.5f * z * (1.f + tanh_<FINE>(0.79788456080286536f * (z + 0.044715f * z * z * z)));
     default: return z;
@@ -84,28 +87,32 @@ template <bool FINE> __device__ __forceinline__ ActD act_d(int a, float z) {
   }
 }
 
-// N at a time, the choice outside
-template <bool FINE, int N> __device__ __forceinline__ void act_n(int a, float (&v)[N]) {
+// N at a time, the choice outside.  ALL: with the GELUs, whose polynomials' constants take some ninety registers inside a loop.
+template <bool FINE, bool ALL, int N> __device__ __forceinline__ void act_n(int a, float (&v)[N]) {
 #define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < N; ++e) v[e] = act_<FINE>(A, v[e]); return;
   switch (a) {
     BLK_CASE(DPVO_ACT_RELU)
     BLK_CASE(DPVO_ACT_SIGMOID)
     BLK_CASE(DPVO_ACT_SILU)
+  }
+  if constexpr (ALL) switch (a) {
     BLK_CASE(DPVO_ACT_GELU)
     BLK_CASE(DPVO_ACT_GELU_TANH)
   }
 #undef BLK_CASE
 }
 // z -> value y and derivative (in z)
-template <bool FINE, int N> __device__ __forceinline__ void act_d_n(int a, float (&z)[N], float (&y)[N]) {
+template <bool FINE, bool ALL, int N> __device__ __forceinline__ void act_d_n(int a, float (&z)[N], float (&y)[N]) {
 #define BLK_CASE(A) case A: _Pragma("unroll") for (int e = 0; e < N; ++e) { const ActD t = act_d<FINE>(A, z[e]); y[e] = t.y; z[e] = t.d; } return;
   switch (a) {
     BLK_CASE(DPVO_ACT_RELU)
     BLK_CASE(DPVO_ACT_SIGMOID)
     BLK_CASE(DPVO_ACT_SILU)
+    BLK_CASE(DPVO_ACT_IDENTITY)
+  }
+  if constexpr (ALL) switch (a) {
     BLK_CASE(DPVO_ACT_GELU)
     BLK_CASE(DPVO_ACT_GELU_TANH)
-    BLK_CASE(DPVO_ACT_IDENTITY)
   }
 #undef BLK_CASE
 }

@@ -13,8 +13,6 @@
 #pragma once
 #include "blocks_dev.h"
 
-#define BLK_INLINE __attribute__((always_inline))
-
 namespace blk {
 namespace {
 
@@ -370,7 +368,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
           } else {
             float g[8], y[8];
             load_n<float, 8>(P.save0 + m * N + n, nv, g);
-            act_d_n<FINE, 8>(act, g, y);
+            act_d_n<FINE, true, 8>(act, g, y);
             if (P.save1) {
               load_n<float, 8>(P.save1 + m * N + n, nv, u);
 #pragma unroll
@@ -394,7 +392,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
             for (int e = 0; e < 8; ++e) v[e] += t[e];
           }
           if (P.save0) store_n<float, 8>(P.save0 + m * N + n, nv, v);
-          act_n<FINE, 8>(act, v);
+          act_n<FINE, true, 8>(act, v);
           if constexpr (PAIR) {
             if (P.bias1) {
               load_n<T, 8>((const T*)P.bias1 + n, nv, t);
@@ -545,7 +543,7 @@ template <int EPI, int MT, int W> __global__ void __launch_bounds__(64 * W) __at
       float* save = j ? P.save1 : P.save0;
       if (save) store_n<float, 4>(save + m * N + n, nv, v[j]);
     }
-    act_n<FINE, 4>(P.act, v[0]);
+    act_n<FINE, true, 4>(P.act, v[0]);
     if constexpr (NA == 2) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[0][e] *= v[1][e];

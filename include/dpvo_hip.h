@@ -635,7 +635,7 @@ int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, size_t ws_by
 /* s = x + scale * act(gate) * post(f);  h = norm(s).   Norms: LAYER (x - mean) / sqrt(var + eps) * w + b, RMS x / sqrt(mean x^2 + eps) * w + b.
  *   x, s [M,D] in x_dtype; f [M,D] and gate [groups,D] in f_dtype (f == NULL: s = x; gate == NULL: no factor; row m reads gate row
  *   m / (M / groups)); w, b, pw, pb [D] in w_dtype or NULL; h [M,D] in h_dtype, x_dtype or f_dtype; s, h contiguous; s may be NULL.
- *   x_dtype is f_dtype or DPVO_F32.  1 <= D <= 16384.  norm == NONE: h is not written.
+ *   x_dtype is f_dtype or DPVO_F32.  gate_activation: IDENTITY, RELU, SIGMOID or SILU.  1 <= D <= 16384.  norm == NONE: h is not written.
  * backward: ds, dh (NULL: zero) -> dx (x_dtype), df, dgate (f_dtype), dw, db, dpw, dpb (w_dtype), each NULL if not wanted, contiguous. */
 #define DPVO_NORM_NONE 0
 #define DPVO_NORM_LAYER 1

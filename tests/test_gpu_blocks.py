@@ -378,11 +378,11 @@ def residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, us
     ((2, 20), 384, "layer", "layer", (2, 20), "silu", 0.5, "sh"),
     ((3, 70), 129, "rms", "rms", (3, 1), "identity", 0.5, "sh"),
     ((600, 2), 65, "rms", None, (600, 1), "sigmoid", 2.0, "sh"),
-    ((5, 4, 3), 520, "layer", "rms", (5, 1, 1), "gelu", -1.0, "sh"),
+    ((5, 4, 3), 520, "layer", "rms", (5, 1, 1), "silu", -1.0, "sh"),
     ((130,), 100, None, "layer", (1,), "relu", 1.0, "sh"),
     ((66,), 1100, "rms", "layer", (66,), "sigmoid", 1.0, "h"),
     ((66,), 40, "rms", "layer", (), "sigmoid", 1.0, "s"),
-    ((9,), 4097, "layer", "rms", (1,), "gelu_tanh", 1.0, "sh"),
+    ((9,), 4097, "layer", "rms", (1,), "sigmoid", 1.0, "sh"),
     ((4,), 8000, "rms", "layer", (4,), "sigmoid", 1.0, "sh"),
     ((3,), 16383, "layer", "layer", (3,), "identity", 1.0, "sh"),
 ])
