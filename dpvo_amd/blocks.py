@@ -68,6 +68,9 @@ def _features(what, x):
 # ------------------------------------------------------------------------------------------------------------------ launches
 def _rows(t):
     """[..., K] as rows whose elements are contiguous: (tensor [M,K], leading dimension); a copy only where no such view exists"""
+    if t.is_contiguous():
+        K = t.shape[-1]
+        return t if t.dim() == 2 else t.view(-1 if K else t.numel(), K), K
     K = t.shape[-1]
     if t.dim() != 2:
         M = 1
@@ -100,11 +103,17 @@ class _Here:
 
 
 _HERE = _Here()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _on(device):
-    """context: the current device is the tensors'"""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on(x):
+    """context: the current device is x's"""
+    return _HERE if x.get_device() == _current_device() else torch.cuda.device(x.device)
+
+
+def _stream(x):
+    return _raw_stream(x.get_device())
 
 
 def _scratch(nbytes, device):
@@ -133,7 +142,7 @@ def _forward(x, wg, bg, act, v=None, wu=None, bu=None, residual=None, save=False
     su = torch.empty(M, N, dtype=torch.float32, device=x.device) if save and wu is not None else None
     p = L.GatedLinear(_p(x), _p(v) if wu is not None else None, _p(wg), _p(wu), _p(bg), _p(bu), _p(residual), _p(y), _p(sg), _p(su), ldx, ldv,
                       ldwg, ldwu, ldr, N, M, N, x.shape[1], Kv, _DTYPES[x.dtype], act)
-    rc = L.lib().dpvo_gated_linear(ctypes.byref(p), L.stream())
+    rc = L.lib().dpvo_gated_linear(ctypes.byref(p), _stream(x))
     if rc:
         L.check(rc, "dpvo_gated_linear")
     return y, sg, su
@@ -144,7 +153,7 @@ def _dact(dy, gate, up, act):
     M, N = dy.shape
     dg = torch.empty(M, N, dtype=dy.dtype, device=dy.device)
     du = torch.empty_like(dg) if up is not None else None
-    L.check(L.lib().dpvo_gated_linear_dact(_p(dy), ld, _p(gate), _p(up), _p(dg), _p(du), N, _DTYPES[dy.dtype], act, M, N, L.stream()),
+    L.check(L.lib().dpvo_gated_linear_dact(_p(dy), ld, _p(gate), _p(up), _p(dg), _p(du), N, _DTYPES[dy.dtype], act, M, N, _stream(dy)),
             "dpvo_gated_linear_dact")
     return dg, du
 
@@ -171,7 +180,7 @@ def _dx(pairs, addend=None, gate=None, up=None, mask=None, act=0):
     lib = L.lib()
     n = lib.dpvo_gated_linear_dx_workspace_bytes(ctypes.byref(p))
     ws = _scratch(n, ref.device)
-    L.check(lib.dpvo_gated_linear_dx(ctypes.byref(p), _p(ws), n, L.stream()), "dpvo_gated_linear_dx")
+    L.check(lib.dpvo_gated_linear_dx(ctypes.byref(p), _p(ws), n, _stream(ref)), "dpvo_gated_linear_dx")
     return dx, dx2
 
 
@@ -197,7 +206,7 @@ def _dw(jobs):
         lib = L.lib()
         n = lib.dpvo_gated_linear_dw_workspace_bytes(ctypes.byref(p))
         ws = _scratch(n, keep[0].device)
-        L.check(lib.dpvo_gated_linear_dw(ctypes.byref(p), _p(ws), n, L.stream()), "dpvo_gated_linear_dw")
+        L.check(lib.dpvo_gated_linear_dw(ctypes.byref(p), _p(ws), n, _stream(keep[0])), "dpvo_gated_linear_dw")
     return out
 
 
@@ -218,7 +227,7 @@ def _shape(g, like):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act):
-        with _on(x.device):
+        with _on(x):
             y, pre, _ = _forward(x, w, b, act, save=act != 0)
         ctx.save_for_backward(x, w, pre)
         ctx.act, ctx.shape = act, x.shape
@@ -229,7 +238,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
-        with _on(x.device):
+        with _on(x):
             dy = _rows(dy)[0]
             d = dy if ctx.act == 0 else _dact(dy, pre, None, ctx.act)[0]
             dx = _dx([(d, w)])[0] if need[0] else None
@@ -247,7 +256,7 @@ def linear(x, weight, bias=None, activation="identity"):
     L.require_cuda(x)
     if _wants_grad(x, weight, bias):
         return _Linear.apply(x, weight, bias, act)
-    with _on(x.device):
+    with _on(x):
         return _like(_forward(x, weight, bias, act)[0], x, weight.shape[0])
 
 
@@ -255,7 +264,7 @@ def linear(x, weight, bias=None, activation="identity"):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, bg, bu, v, residual, act):
-        with _on(x.device):
+        with _on(x):
             y, g, u = _forward(x, wg, bg, act, v, wu, bu, residual, save=True)
         ctx.save_for_backward(x, v, wg, wu, g, u)
         ctx.act = act
@@ -267,7 +276,7 @@ class _GatedLinear(torch.autograd.Function):
         x, v, wg, wu, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dv = dwg = dwu = dbg = dbu = None
-        with _on(x.device):
+        with _on(x):
             if any(need[:6]):
                 dg, du = _dact(dy, g, u, ctx.act)
                 if v is None:
@@ -300,7 +309,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu", up_
     L.require_cuda(x)
     if _wants_grad(x, w_gate, w_up, b_gate, b_up, up_input, residual):
         return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, up_input, residual, act)
-    with _on(x.device):
+    with _on(x):
         return _like(_forward(x, w_gate, b_gate, act, up_input, w_up, b_up, residual)[0], x, w_gate.shape[0])
 
 
@@ -308,7 +317,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu", up_
 class _FeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, bg, bu, bd, act):
-        with _on(x.device):
+        with _on(x):
             h, g, u = _forward(x, wg, bg, act, None, wu, bu, save=True)
             y = _forward(h, wd, bd, 0)[0]
         ctx.save_for_backward(x, wg, wu, wd, h, g, u)
@@ -321,7 +330,7 @@ class _FeedForward(torch.autograd.Function):
         x, wg, wu, wd, h, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dwu = dbg = dbu = None
-        with _on(x.device):
+        with _on(x):
             dy = _rows(dy)[0]
             jobs = [(dy, h, need[3], need[6])]
             if any(need[i] for i in (0, 1, 2, 4, 5)):
@@ -351,7 +360,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     L.require_cuda(x)
     if _wants_grad(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
         return _FeedForward.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
-    with _on(x.device):
+    with _on(x):
         h = _forward(x, w_gate, b_gate, act, None, w_up, b_up)[0]
         return _like(_forward(h, w_down, b_down, 0)[0], x, w_down.shape[0])
 
@@ -363,7 +372,7 @@ _RELU, _SIGMOID = ACTIVATIONS["relu"], ACTIVATIONS["sigmoid"]
 class _GatedResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, bg, w1, b1, w2, b2):
-        with _on(x.device):
+        with _on(x):
             t = _forward(x, w1, b1, _RELU)[0]
             y, g, r = _forward(x, wg, bg, _SIGMOID, t, w2, b2, residual=x, save=True)
         ctx.save_for_backward(x, wg, w1, w2, t, g, r)
@@ -375,7 +384,7 @@ class _GatedResidual(torch.autograd.Function):
         x, wg, w1, w2, t, g, r = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dbg = dw1 = db1 = dw2 = db2 = None
-        with _on(x.device):
+        with _on(x):
             dy = _rows(dy)[0]
             dg, dr = _dact(dy, g, r, _SIGMOID)
             # the ReLU's derivative is where its output is positive: the gradient of its input is masked in the product's epilogue
@@ -406,7 +415,7 @@ def gated_residual(x, w_gate, b_gate, w_in, b_in, w_out, b_out):
     L.require_cuda(x)
     if _wants_grad(x, w_gate, b_gate, w_in, b_in, w_out, b_out):
         return _GatedResidual.apply(x, w_gate, b_gate, w_in, b_in, w_out, b_out)
-    with _on(x.device):
+    with _on(x):
         t = _forward(x, w_in, b_in, _RELU)[0]
         return _like(_forward(x, w_gate, b_gate, _SIGMOID, t, w_out, b_out, residual=x)[0], x, D)
 
@@ -429,7 +438,8 @@ def _norm_struct(x, f, gate, w, b, pw, pb, cfg, s, h, ds, dh, grads):
     hd = _DTYPES[h_dtype]
     par = w if w is not None else b if b is not None else pw if pw is not None else pb
     M, D = x.shape
-    p = L.ResidualNorm(x.data_ptr(), _p(f), _p(gate), _p(w), _p(b), _p(pw), _p(pb), _p(s), _p(h), _p(ds), _p(dh), *map(_p, grads), ldx, ldf, ldg,
+    p = L.ResidualNorm(x.data_ptr(), _p(f), _p(gate), _p(w), _p(b), _p(pw), _p(pb), _p(s), _p(h), _p(ds), _p(dh),
+                       *(grads if grads is _NO_GRADS else map(_p, grads)), ldx, ldf, ldg,
                        ldds, lddh, M, groups, D, _DTYPES[x.dtype], hd if f is None else _DTYPES[f.dtype], hd,
                        L.F32 if par is None else _DTYPES[par.dtype], norm_k, post_k, gate_act, scale, eps, post_eps)
     return p, (x, f, gate, w, b, pw, pb, ds, dh)
@@ -438,13 +448,20 @@ def _norm_struct(x, f, gate, w, b, pw, pb, cfg, s, h, ds, dh, grads):
 _NO_GRADS = (None,) * 7
 
 
+def _new(x, dtype):
+    """contiguous, of x's shape"""
+    if dtype == x.dtype and x.is_contiguous():
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
+
+
 def _norm_forward(x, f, gate, w, b, pw, pb, cfg):
     """-> s (None without a branch), h (None without a norm)"""
-    with _on(x.device):
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if f is not None else None
-        h = torch.empty(x.shape, dtype=cfg[6], device=x.device) if cfg[0] else None
+    with _on(x):
+        s = _new(x, x.dtype) if f is not None else None
+        h = _new(x, cfg[6]) if cfg[0] else None
         p, keep = _norm_struct(x, f, gate, w, b, pw, pb, cfg, s, h, None, None, _NO_GRADS)
-        rc = L.lib().dpvo_residual_norm(ctypes.byref(p), L.stream())
+        rc = L.lib().dpvo_residual_norm(ctypes.byref(p), _stream(x))
     if rc:
         L.check(rc, "dpvo_residual_norm")
     return s, h
@@ -466,7 +483,7 @@ class _ResidualNorm(torch.autograd.Function):
         grads = [None] * 7
         if ds is None and dh is None:
             return (*grads, None)
-        with _on(x.device):
+        with _on(x):
             make = torch.empty if x.numel() else torch.zeros
             for i, t in enumerate((x, f, gate, w, b, pw, pb)):
                 if t is not None and ctx.needs_input_grad[i]:
@@ -476,12 +493,14 @@ class _ResidualNorm(torch.autograd.Function):
                 lib = L.lib()
                 n = lib.dpvo_residual_norm_backward_workspace_bytes(ctypes.byref(p))
                 ws = _scratch(n, x.device)
-                L.check(lib.dpvo_residual_norm_backward(ctypes.byref(p), _p(ws), n, L.stream()), "dpvo_residual_norm_backward")
+                L.check(lib.dpvo_residual_norm_backward(ctypes.byref(p), _p(ws), n, _stream(x)), "dpvo_residual_norm_backward")
         return (*grads, None)
 
 
 def _gate_rows(what, x, gate):
     """how many rows of `gate` there are: it is shaped like x, or with ones (or nothing) in the place of x's last leading dimensions"""
+    if gate.dim() == 1 and gate.shape[0] == x.shape[-1]:
+        return 1
     lead = [1] * (x.dim() - gate.dim()) + list(gate.shape[:-1])
     if gate.dim() > x.dim() or gate.dim() < 1 or gate.shape[-1] != x.shape[-1]:
         _fail(what, f"gate {tuple(gate.shape)} does not go with x {tuple(x.shape)}")

@@ -165,7 +165,11 @@ template <int L, int V, int E, bool FINE> struct Row {
     a = kind == DPVO_NORM_LAYER ? a * inv : 0.f;
     b *= inv;
 #pragma unroll
-    for (int e = 0; e < P; ++e) d[e] = r * (d[e] - a - xh[e] * b);
+    for (int i = 0; i < V; ++i) {
+      const bool in = has(i);                            // (behind D the mean alone would be left, and reach the next sum)
+#pragma unroll
+      for (int e = i * E; e < (i + 1) * E; ++e) d[e] = in ? r * (d[e] - a - xh[e] * b) : 0.f;
+    }
   }
 };
 

@@ -385,6 +385,11 @@ def residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, us
     ((9,), 4097, "layer", "rms", (1,), "sigmoid", 1.0, "sh"),
     ((4,), 8000, "rms", "layer", (4,), "sigmoid", 1.0, "sh"),
     ((3,), 16383, "layer", "layer", (3,), "identity", 1.0, "sh"),
+    # lanes without a column (D is no multiple of a row's lanes) beside a gate that is not 0 there: their mean must not reach the branch's sums
+    ((5,), 671, "layer", "layer", (5,), "sigmoid", 1.0, "sh"),
+    ((9,), 384, "layer", "layer", (), "sigmoid", 1.0, "sh"),
+    ((6,), 2560, "layer", "layer", (6,), "sigmoid", 0.5, "sh"),
+    ((3,), 10000, "layer", "layer", (3,), "sigmoid", 1.0, "h"),
 ])
 def test_residual_norm(dev, tx, tb, lead, D, kind, post, gate, gate_act, scale, use):
     g = torch.Generator().manual_seed(D + len(lead))
