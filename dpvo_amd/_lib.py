@@ -34,7 +34,7 @@ SYMBOLS = [
     "dpvo_normalize_image", "dpvo_patch_colors", "dpvo_store_features", "dpvo_append_edges", "dpvo_gather_edges", "dpvo_gather_edges2",
     "dpvo_motion_model", "dpvo_median_depth", "dpvo_frame_patches", "dpvo_frame_state", "dpvo_frame_state_part", "dpvo_keyframe_step", "dpvo_frame_update", "dpvo_debug_stamp",
     "dpvo_encoders_workspace_bytes", "dpvo_encoders_forward", "dpvo_encoders_forward_hold", "dpvo_pool4_nhwc",
-    "dpvo_gated_linear", "dpvo_gated_linear_dact", "dpvo_gated_linear_dx_workspace_bytes", "dpvo_gated_linear_dx",
+    "dpvo_gated_linear_workspace_bytes", "dpvo_gated_linear", "dpvo_gated_linear_dact", "dpvo_gated_linear_dx_workspace_bytes", "dpvo_gated_linear_dx",
     "dpvo_gated_linear_dw_workspace_bytes", "dpvo_gated_linear_dw",
     "dpvo_residual_norm", "dpvo_residual_norm_backward_workspace_bytes", "dpvo_residual_norm_backward",
 ]
@@ -152,14 +152,13 @@ def lib():
                 raise DPVOHipError(f"libdpvo_hip.so does not export {s}")
         for s in ("dpvo_plan_workspace_bytes", "dpvo_plan_wide_workspace_bytes", "dpvo_normalize_scratch_bytes", "dpvo_neighbors_workspace_bytes", "dpvo_ba_workspace_bytes",
                   "dpvo_gba_workspace_bytes", "dpvo_gba_solve_workspace_bytes", "dpvo_solve_system_workspace_bytes", "dpvo_encoders_workspace_bytes",
-                  "dpvo_update_fused_workspace_bytes", "dpvo_update_fused_pack_bytes", "dpvo_gated_linear_dx_workspace_bytes",
+                  "dpvo_update_fused_workspace_bytes", "dpvo_update_fused_pack_bytes", "dpvo_gated_linear_workspace_bytes", "dpvo_gated_linear_dx_workspace_bytes",
                   "dpvo_gated_linear_dw_workspace_bytes", "dpvo_residual_norm_backward_workspace_bytes"):
             getattr(L, s).restype = ctypes.c_size_t
         vp, i64_, i32_ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
-        L.dpvo_gated_linear.argtypes = [vp, vp]
         L.dpvo_gated_linear_dact.argtypes = [vp, i64_, vp, vp, vp, vp, i64_, i32_, i32_, i64_, i64_, vp]
-        L.dpvo_gated_linear_dx_workspace_bytes.argtypes = L.dpvo_gated_linear_dw_workspace_bytes.argtypes = L.dpvo_residual_norm_backward_workspace_bytes.argtypes = [vp]
-        L.dpvo_gated_linear_dx.argtypes = L.dpvo_gated_linear_dw.argtypes = L.dpvo_residual_norm_backward.argtypes = [vp, vp, ctypes.c_size_t, vp]
+        L.dpvo_gated_linear_workspace_bytes.argtypes = L.dpvo_gated_linear_dx_workspace_bytes.argtypes = L.dpvo_gated_linear_dw_workspace_bytes.argtypes = L.dpvo_residual_norm_backward_workspace_bytes.argtypes = [vp]
+        L.dpvo_gated_linear.argtypes = L.dpvo_gated_linear_dx.argtypes = L.dpvo_gated_linear_dw.argtypes = L.dpvo_residual_norm_backward.argtypes = [vp, vp, ctypes.c_size_t, vp]
         L.dpvo_residual_norm.argtypes = [vp, vp]
         L.dpvo_abi_version.restype = ctypes.c_int
         if L.dpvo_abi_version() != ABI_VERSION:

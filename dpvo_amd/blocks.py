@@ -142,7 +142,11 @@ def _forward(x, wg, bg, act, v=None, wu=None, bu=None, residual=None, save=False
     su = torch.empty(M, N, dtype=torch.float32, device=x.device) if save and wu is not None else None
     p = L.GatedLinear(_p(x), _p(v) if wu is not None else None, _p(wg), _p(wu), _p(bg), _p(bu), _p(residual), _p(y), _p(sg), _p(su), ldx, ldv,
                       ldwg, ldwu, ldr, N, M, N, x.shape[1], Kv, _DTYPES[x.dtype], act)
-    rc = L.lib().dpvo_gated_linear(ctypes.byref(p), _stream(x))
+    lib, n, ws = L.lib(), 0, None
+    if act == 0 and wu is None:
+        n = lib.dpvo_gated_linear_workspace_bytes(ctypes.byref(p))
+        ws = _scratch(n, x.device)
+    rc = lib.dpvo_gated_linear(ctypes.byref(p), _p(ws), n, _stream(x))
     if rc:
         L.check(rc, "dpvo_gated_linear")
     return y, sg, su

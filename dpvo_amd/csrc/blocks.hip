@@ -21,12 +21,14 @@ int gemm(const GemmArgs& a, int dtype, int form, int epi, int kind, int64_t tile
 }
 inline int block_k(int dtype) { return dtype == DPVO_F32 ? 32 : 64; }
 
-// out[e] = sum over parts of part[i][e] (+ addend[e]), all contiguous; a job for each row of the grid
+// out[e] = sum over parts of part[i][e] (+ bias[e % N]) (+ addend[e]), all contiguous; a job for each row of the grid
 struct SumJob {
   const float* part;
   int64_t size;
   const void* addend;
   void* out;
+  const void* bias;
+  int64_t N;
 };
 struct SumArgs {
   SumJob j[2 * MAXP];
@@ -42,6 +44,14 @@ template <class T> __global__ void __launch_bounds__(256) split_sum_kernel(const
     load_n<float, 4>(j.part + s * j.size + e, nv, t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += t[i];
+  }
+  if (j.bias) {
+    int64_t n = e % j.N;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < nv) v[i] += (float)((const T*)j.bias)[n];
+      n = n + 1 < j.N ? n + 1 : 0;
+    }
   }
   if (j.addend) {
     load_n<T, 4>((const T*)j.addend + e, nv, t);
@@ -151,27 +161,31 @@ struct Plan {
   int kind;
   int64_t splits;
 };
-inline int tile_size(int kind) { return kind == T_BIG ? 256 : kind == T_SMALL ? 64 : 128; }
+inline int tile_size(int kind) { return kind == T_BIG ? 256 : kind == T_SMALL || kind == T_TINY ? 64 : 128; }
 // `count(t)`: tiles of t x t; nb: blocks of the summed index; cut: whether parts are possible.
-// 256 x 256 reads LDS least per product and gives 1095 Tflop/s (bf16, 8192 x 8192 x 4096) where 128 x 128 gives 885; but only one workgroup
-// fits a compute unit, so its epilogue hides behind nothing: with 16 blocks it still wins (79.7 against 89.3 us, 4096 x 4096 x 1024 twice),
-// with 6 it loses (65.2 against 56.6 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
-// 128 x 128 wants two workgroups on a compute unit: at 432 tiles it wins over 64 x 64 (15.7 against 20.6 us), at 256 it loses (19.1 against 18.0).
+//  - 256 x 256 reads LDS least per product and gives 1095 Tflop/s (bf16, 8192 x 8192 x 4096) where 128 x 128 gives 885, so a round of the latter (two
+//    workgroups on each of 256 compute units) takes 0.62 of a round of the former (one): whichever needs less.  But nothing hides the epilogue of
+//    one workgroup alone: with 16 blocks it still wins (79.7 against 89.3 us, 4096 x 4096 x 1024 twice), with 6 or 12 it loses (65.2 against
+//    56.6 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
+//  - 128 x 128 wants its two workgroups: at 432 tiles it wins over 64 x 64 (15.7 against 20.6 us), at 256 it loses (19.1 against 18.0).
+//  - Parts: towards two workgroups a compute unit, each with 12 blocks at least (a part costs a tile's write and read in f32, and all of them a
+//    launch); dw 384 x 384 over 45312 rows: 45 us in 56 parts, 56 in 64, 59 in 16.  Where that does not fill them, small tiles in parts of 4
+//    blocks at least: over 9216 rows 23 us in 21 parts, 25 with large tiles in 16.  Below 16 blocks a second launch costs more than it
+//    saves: 333 x 2048 x 768 8.6 us whole, 14.0 in three.
+//  - 64 x 64 by four waves where there are few: 1237 x 385 x 882 in f32 24 us against 40 with two waves, at 864 tiles 13.3 against 11.6.
 template <class F> Plan plan(F count, int64_t nb, int dtype, bool cut) {
-  if (dtype != DPVO_F32 && nb >= 12 && count(256) >= 200) return {T_BIG, 1};
   const int64_t t = count(128);
+  if (dtype != DPVO_F32 && nb >= 16 && cdiv64(count(256), 256) * 100 < cdiv64(t, 512) * 62) return {T_BIG, 1};
   if (t >= 384) return {T_TILE, 1};
-  if (!cut || t == 0) return {T_SMALL, 1};
-  // parts: towards two workgroups on each of 256 compute units, each with 8 blocks at least (a part costs a tile's write and read in f32);
-  // where that does not even give one each, small tiles with 4 blocks at least.  dw 384 x 384 over 45312 rows: 45 us in 56 parts, 56 in 64 and
-  // 59 in 16; over 9216: 23 us with small tiles in 21, 25 with large ones in 16.
+  const int small = count(64) >= 640 ? T_SMALL : T_TINY;
+  if (!cut || t == 0 || nb < 16) return {small, 1};
   auto parts = [&](int64_t want, int64_t least) {
     const int64_t n = want < nb / least ? want : nb / least;
     return n < 1 ? 1 : n > 64 ? 64 : n;
   };
-  const int64_t n = parts(512 / t, 8);
-  if (n * t >= 256) return {T_TILE, n};
-  return {T_SMALL, parts(768 / count(64), 4)};
+  const int64_t n = parts(512 / t, 12);
+  if (n * t >= 384) return {T_TILE, n};
+  return {small, parts(768 / count(64), 4)};
 }
 inline int64_t tiles(int64_t M, int64_t N, int t) { return cdiv64(M, t) * cdiv64(N, t); }
 int64_t tiles_of(Prob& p, int kind, int halves = 1) {
@@ -230,14 +244,35 @@ int norm_run(const NormArgs& a, int sh, bool back, int64_t blocks, hipStream_t s
 
 using namespace blk;
 
-extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream) {
+// A plain projection (no activation, nothing saved) of more rows than the few-row kernel takes may be cut into parts like a gradient's sum
+static Plan linear_plan(const dpvo_gated_linear_t* p, int epi) {
+  const int bk = block_k(p->dtype);
+  const bool cut = epi == E_LIN && p->activation == DPVO_ACT_IDENTITY && !p->save_gate && p->ldy == p->N && (!p->residual || p->ldr == p->N);
+  Plan c = plan([&](int t) { return tiles(p->M, epi == E_GATE ? 2 * p->N : p->N, t); }, cdiv64(p->K, bk) + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0),
+                p->dtype, cut);
+  if (epi == E_GATE2 && c.kind == T_BIG) c.kind = T_TILE;      // (two sets of sums do not fit the registers of the largest tile)
+  return c;
+}
+static int linear_epi(const dpvo_gated_linear_t* p) {
+  if (!p->w_up) return E_LIN;
+  return p->v == p->x && p->ldv == p->ldx && p->Kv == p->K ? E_GATE : E_GATE2;
+}
+
+extern "C" size_t dpvo_gated_linear_workspace_bytes(const dpvo_gated_linear_t* p) {
+  if (!p || !type_ok(p->dtype) || p->M <= FEW_ROWS || p->N <= 0 || p->K < 0 || p->Kv < 0 || p->w_up) return 0;
+  const Plan c = linear_plan(p, E_LIN);
+  return c.splits > 1 ? (size_t)(c.splits * p->M * p->N * 4) : 0;
+}
+
+extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* ws, size_t ws_bytes, void* stream) {
   if (!p || !type_ok(p->dtype) || !act_ok(p->activation) || p->M < 0 || p->N < 0 || p->K < 0 || p->Kv < 0) return DPVO_E_INVALID;
   if (p->M == 0 || p->N == 0) return DPVO_OK;
   const int size = type_size(p->dtype);
   if (!p->y || (p->K && (!p->x || !p->w_gate)) || (p->w_up && p->Kv && !p->v)) return DPVO_E_INVALID;
   if (!ld_ok(p->ldx, p->K, size) || !ld_ok(p->ldwg, p->K, size) || p->ldy < p->N || (p->residual && p->ldr < p->N)) return DPVO_E_INVALID;
   if (p->w_up && (!ld_ok(p->ldv, p->Kv, size) || !ld_ok(p->ldwu, p->Kv, size))) return DPVO_E_INVALID;
-  const bool same = p->w_up && p->v == p->x && p->ldv == p->ldx && p->Kv == p->K;
+  hipStream_t s = (hipStream_t)stream;
+  const int bk = block_k(p->dtype), epi = linear_epi(p);
   GemmArgs a = {};
   a.n = 1;
   Prob& q = a.p[0];
@@ -247,14 +282,21 @@ extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream) {
   q.bias0 = p->b_gate; q.bias1 = p->b_up; q.addend = p->residual; q.ldadd = p->ldr;
   q.out0 = p->y; q.ldo = p->ldy; q.save0 = p->save_gate; q.save1 = p->w_up ? p->save_up : nullptr;
   q.act = p->activation; q.splits = 1;
-  const int bk = block_k(p->dtype), epi = !p->w_up ? E_LIN : same ? E_GATE : E_GATE2;
   q.nb0 = cdiv64(p->K, bk);
   q.nb = q.nb0 + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0);
-  if (p->M <= FEW_ROWS) return gemm(a, p->dtype, F_NT, epi, T_FEW, cdiv64(p->N, 16), (hipStream_t)stream);
-  int kind = plan([&](int t) { return tiles(p->M, epi == E_GATE ? 2 * p->N : p->N, t); }, q.nb, p->dtype, false).kind;
-  if (epi == E_GATE2 && kind == T_BIG) kind = T_TILE;    // (two sets of sums do not fit the registers of the largest tile)
-  const int64_t n = tiles_of(q, kind, epi == E_GATE ? 2 : 1);
-  return gemm(a, p->dtype, F_NT, epi, kind, n, (hipStream_t)stream);
+  if (p->M <= FEW_ROWS) return gemm(a, p->dtype, F_NT, epi, T_FEW, cdiv64(p->N, 16), s);
+  const Plan c = linear_plan(p, epi);
+  const int64_t n = tiles_of(q, c.kind, epi == E_GATE ? 2 : 1);
+  if (c.splits == 1) return gemm(a, p->dtype, F_NT, epi, c.kind, n, s);
+  if ((size_t)(c.splits * p->M * p->N * 4) > ws_bytes || !ws) return DPVO_E_WORKSPACE;
+  q.splits = (int)c.splits;
+  q.part = (float*)ws;
+  const int rc = gemm(a, p->dtype, F_NT, epi, c.kind, n * c.splits, s);
+  SumArgs sum = {};
+  sum.n = 1;
+  sum.splits = q.splits;
+  sum.j[0] = {q.part, p->M * p->N, p->residual, p->y, p->b_gate, p->N};
+  return rc ? rc : split_sum(sum, p->dtype, s);
 }
 
 extern "C" int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, const float* up, void* d_gate, void* d_up, int64_t ldo, int dtype,
@@ -325,7 +367,7 @@ extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, s
     SumArgs sum = {};
     sum.n = 1;
     sum.splits = q.splits;
-    sum.j[0] = {q.part, p->M * p->N, p->addend, p->dx};
+    sum.j[0] = {q.part, p->M * p->N, p->addend, p->dx, nullptr, 0};
     return rc ? rc : split_sum(sum, p->dtype, s);
   }
   q.addend = p->addend; q.ldadd = p->ldadd;
@@ -382,10 +424,10 @@ extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, s
     q.splits = (int)splits;
     q.out0 = p->dw[i]; q.ldo = p->K[i]; q.colsum = p->db[i];
     if (splits > 1) {
-      sum.j[sum.n++] = {q.part = w, q.M * q.N, nullptr, p->dw[i]};
+      sum.j[sum.n++] = {q.part = w, q.M * q.N, nullptr, p->dw[i], nullptr, 0};
       w += splits * q.M * q.N;
       if (p->db[i]) {
-        sum.j[sum.n++] = {w, q.M, nullptr, p->db[i]};
+        sum.j[sum.n++] = {w, q.M, nullptr, p->db[i], nullptr, 0};
         q.colsum = w;
         w += splits * q.M;
       }

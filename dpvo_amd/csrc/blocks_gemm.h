@@ -22,9 +22,12 @@ constexpr int BK = 8 * KE;
 constexpr bool FINE = sizeof(T) == 4;
 
 template <int KIND> struct Cfg;
-template <> struct Cfg<T_TILE> { static constexpr int NT = 256, TM = 128, TN = 128, WN = 2, MI = 2; };
-template <> struct Cfg<T_BIG> { static constexpr int NT = 512, TM = 256, TN = 256, WN = 4, MI = 4; };
-template <> struct Cfg<T_SMALL> { static constexpr int NT = 128, TM = 64, TN = 64, WN = 1, MI = 1; };
+// NT threads; WN wave columns of 64, WK waves that share a block's steps; MI 32-row pieces of a wave.  DEPTH: blocks whose loads are under way
+// (two for the shape that runs alone on its compute unit; for the others two made no difference)
+template <> struct Cfg<T_TILE> { static constexpr int NT = 256, TM = 128, TN = 128, WN = 2, WK = 1, MI = 2, DEPTH = 1; };
+template <> struct Cfg<T_BIG> { static constexpr int NT = 512, TM = 256, TN = 256, WN = 4, WK = 1, MI = 4, DEPTH = 1; };
+template <> struct Cfg<T_SMALL> { static constexpr int NT = 128, TM = 64, TN = 64, WN = 1, WK = 1, MI = 1, DEPTH = 1; };
+template <> struct Cfg<T_TINY> { static constexpr int NT = 256, TM = 64, TN = 64, WN = 1, WK = 2, MI = 1, DEPTH = 2; };
 
 __device__ __forceinline__ int swz(int row, int c) { return row * 128 + ((c ^ (row & 7) ^ ((row >> 3) & 7)) << 4); }
 
@@ -51,107 +54,112 @@ template <int N> __device__ __forceinline__ void raw_guard(const T* p, int64_t n
   }
 }
 
-// One operand's share of a tile: R rows x one block, by NT threads, four 16-byte pieces of registers each.
+// One operand's share of a tile: R rows x one block, by NT threads, NC 16-byte pieces of registers each.
 //   summed index contiguous (row): chunk t % 8 of rows t / 8 + i * NT / 8
-//   summed index as rows (col): columns 4 (t % (R / 4)) .. + 3 of summed indices KE (t / (R / 4)) .. + KE - 1
+//   summed index as rows (col): columns NC (t % (R / NC)) .. + NC - 1 of summed indices KE (t / (R / NC)) .. + KE - 1
 // Whole blocks are loaded through a buffer descriptor whose base moves on (scalar work only) and per-lane offsets that never change;
 // a segment's last blocks through guarded loads.
 template <int R, int NT, bool TR> struct Stage {
-  i4v v[4];
-  static_assert(R * 8 == NT * 4, "four chunks per thread");
+  static constexpr int NC = R * 8 / NT;
+  static_assert(NC == 4 || NC == 2, "pieces per thread");
+  typedef i4v Regs[NC];
   static constexpr int RS = NT / 8;                      // rows between a thread's chunks
-  uint32_t off[TR ? 1 : 4];                              // bytes from the tile's base
+  uint32_t off[TR ? 1 : NC];                             // bytes from the tile's base
   // where the pieces go in the first buffer: rows 64 apart have their chunks alike
-  static constexpr int NL = TR || RS == 16 ? 4 : RS == 32 ? 2 : 1;
+  static constexpr int NL = TR || RS == 16 ? NC : RS == 32 ? 2 : 1;
   uint32_t lds[NL];
 
-  static __device__ __forceinline__ int chunk() { return TR ? (int)threadIdx.x / (R / 4) : (int)threadIdx.x & 7; }
+  static __device__ __forceinline__ int chunk() { return TR ? (int)threadIdx.x / (R / NC) : (int)threadIdx.x & 7; }
   static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x >> 3) + i * RS; }
-  static __device__ __forceinline__ int col() { return (int)threadIdx.x % (R / 4) * 4; }
+  static __device__ __forceinline__ int col() { return (int)threadIdx.x % (R / NC) * NC; }
 
   __device__ __forceinline__ void init_lds(uint32_t base) {
-    if constexpr (TR) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lds[j] = base + swz(col() + j, chunk());
-    } else {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) lds[i] = base + swz(row(i), chunk());
-    }
+    for (int i = 0; i < NL; ++i) lds[i] = base + (TR ? swz(col() + i, chunk()) : swz(row(i), chunk()));
   }
   // row: `at(r)`: element offset of tile row r (clamped to the operand); col: `left`: columns from the tile's first on
   template <class F> __device__ __forceinline__ void aim_rows(F at) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) off[i] = (uint32_t)((at(row(i)) + chunk() * KE) * (int64_t)sizeof(T));
+    for (int i = 0; i < NC; ++i) off[i] = (uint32_t)((at(row(i)) + chunk() * KE) * (int64_t)sizeof(T));
   }
   __device__ __forceinline__ void aim_cols(int64_t ld, int64_t left) {
-    const int64_t last = (left - 1) / 4 * 4;             // groups behind the last column: the last group again, not stored
+    const int64_t last = (left - 1) / NC * NC;           // groups behind the last column: the last group again, not stored
     off[0] = (uint32_t)((chunk() * KE * ld + (col() < last ? col() : last)) * (int64_t)sizeof(T));
   }
   // base: (tile's first row, k), or for the pieces whose bit is set in `other` base1; col: (k, first column).  All scalar.
-  __device__ __forceinline__ void load(const T* base, const T* base1, int other, int64_t ld) {
+  __device__ __forceinline__ void load(Regs& v, const T* base, const T* base1, int other, int64_t ld) const {
     if constexpr (!TR) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NC; ++i) {
         const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)(other >> i & 1 ? base1 : base), 0, -1, 0x27000);
         v[i] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(d, off[i], 0, 0));
       }
     } else {
       const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x27000);
       const uint32_t step = (uint32_t)(ld * sizeof(T));
-      if constexpr (sizeof(T) == 4) {
+      constexpr int W = NC * (int)sizeof(T) / 4;         // dwords of a summed index's columns: 4, 2 or 1
+      int t[KE * W];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(d, off[0], k * step, 0));
-      } else {
+      for (int k = 0; k < KE; ++k) {
+        if constexpr (W == 4) {
+          const i4v x = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(d, off[0], k * step, 0));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {                    // rows 2k, 2k + 1 of the 8 x 4 piece
-          const i2v lo = __builtin_bit_cast(i2v, __builtin_amdgcn_raw_buffer_load_b64(d, off[0], 2 * k * step, 0));
-          const i2v hi = __builtin_bit_cast(i2v, __builtin_amdgcn_raw_buffer_load_b64(d, off[0], (2 * k + 1) * step, 0));
-          v[k] = i4v{lo[0], lo[1], hi[0], hi[1]};
+          for (int w = 0; w < 4; ++w) t[k * 4 + w] = x[w];
+        } else if constexpr (W == 2) {
+          const i2v x = __builtin_bit_cast(i2v, __builtin_amdgcn_raw_buffer_load_b64(d, off[0], k * step, 0));
+          t[k * 2] = x[0];
+          t[k * 2 + 1] = x[1];
+        } else {
+          t[k] = (int)__builtin_amdgcn_raw_buffer_load_b32(d, off[0], k * step, 0);
         }
       }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = i4v{t[i * 4], t[i * 4 + 1], t[i * 4 + 2], t[i * 4 + 3]};
     }
   }
   // the same with zeros for summed indices >= nk (counted from the block's first) and nothing read behind the operand
-  __device__ __forceinline__ void load_guard(const T* base, const T* base1, int other, int64_t ld, int64_t nk, int64_t left) {
+  __device__ __forceinline__ void load_guard(Regs& v, const T* base, const T* base1, int other, int64_t ld, int64_t nk, int64_t left) const {
     if constexpr (!TR) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NC; ++i) {
         T o[KE];
         raw_guard<KE>((const T*)((const char*)(other >> i & 1 ? base1 : base) + off[i]), nk - chunk() * KE, o);
         v[i] = __builtin_bit_cast(i4v, o);
       }
     } else {
       const T* p = base + (int64_t)chunk() * KE * ld + col();
-      T o[KE][4];
+      T o[KE][NC];
 #pragma unroll
-      for (int k = 0; k < KE; ++k) raw_guard<4>(p + k * ld, chunk() * KE + k < nk ? left - col() : 0, o[k]);
-      __builtin_memcpy(v, o, sizeof(v));
+      for (int k = 0; k < KE; ++k) raw_guard<NC>(p + k * ld, chunk() * KE + k < nk ? left - col() : 0, o[k]);
+      __builtin_memcpy(&v, o, sizeof(v));
     }
   }
   // adds this thread's share of the columns' sums
-  __device__ __forceinline__ void add_cols(float (&sum)[4]) const {
-    T o[KE][4];
-    __builtin_memcpy(o, v, sizeof(o));
+  static __device__ __forceinline__ void add_cols(const Regs& v, float (&sum)[NC]) {
+    T o[KE][NC];
+    __builtin_memcpy(o, &v, sizeof(o));
 #pragma unroll
     for (int k = 0; k < KE; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] += (float)o[k][j];
+      for (int j = 0; j < NC; ++j) sum[j] += (float)o[k][j];
   }
-  __device__ __forceinline__ void store(char* buf, uint32_t flip) const {
+  __device__ __forceinline__ void store(const Regs& v, char* buf, uint32_t flip) const {
     if constexpr (!TR) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *(i4v*)(buf + ((lds[i % NL] + i / NL * NL * RS * 128) ^ flip)) = v[i];
+      for (int i = 0; i < NC; ++i) *(i4v*)(buf + ((lds[i % NL] + i / NL * NL * RS * 128) ^ flip)) = v[i];
     } else {
+      constexpr int W = NC * (int)sizeof(T) / 4;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NC; ++j) {
         i4v d;
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) d[k] = v[k][j];
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)                    // dwords j / 2 of rows 2k and 2k + 1
-            d[k] = (int)__builtin_amdgcn_perm((unsigned)v[k][2 + j / 2], (unsigned)v[k][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 4) {
+            d[k] = v[(k * W + j) / 4][(k * W + j) % 4];
+          } else {                                       // column j of summed indices 2k and 2k + 1
+            const int lo = 2 * k * W + j / 2, hi = lo + W;
+            d[k] = (int)__builtin_amdgcn_perm((unsigned)v[hi / 4][hi % 4], (unsigned)v[lo / 4][lo % 4], j & 1 ? 0x07060302u : 0x05040100u);
+          }
         }
         *(i4v*)(buf + (lds[j] ^ flip)) = d;
       }
@@ -165,7 +173,9 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   constexpr bool TA = FORM == F_TN, TB = FORM != F_NT;
   constexpr bool TWO = EPI == E_GATE2;                   // two accumulators, one after the other
   constexpr uint32_t HALF = (TM + TN) * 128;             // one buffer; a power of two, so that an XOR turns to the other
-  __shared__ __attribute__((aligned(16))) char lds[2 * HALF];
+  constexpr int PITCH = 68;                              // epilogue: floats of a row of 64; 272 bytes, so that 8 rows' pieces lie in different banks
+  constexpr uint32_t STAGING = NT / 64 * 32 * PITCH * 4;
+  __shared__ __attribute__((aligned(16))) char lds[2 * HALF > STAGING ? 2 * HALF : STAGING];
 
   // ---- which tile.  Workgroups go to the 8 dies in turn: die x takes the x-th eighth of the tiles, so that tiles that share rows or columns
   // share an L2; within it, 8 row tiles at a time.
@@ -192,7 +202,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   const int64_t M = P.M, N = P.N;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / C::WN, wn = wave % C::WN;
+  const int wk = wave % C::WK, wn = wave / C::WK % C::WN, wm = wave / (C::WK * C::WN);
   const int lr = lane & 31, lh = lane >> 5;
 
   // ---- operands
@@ -206,7 +216,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   int other = 0;
   if constexpr (EPI == E_GATE)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) other |= ((wave * 8 + i * (NT / 8)) >> 5 & 1) << i;
+    for (int i = 0; i < sb.NC; ++i) other |= ((wave * 8 + i * (NT / 8)) >> 5 & 1) << i;
   // a tile that hangs over the last column of a col operand: its last group of four may read up to three elements into the rows that follow,
   // which must exist
   const int spare = (TA && m0 + TM > M) || (TB && n0 + TN > N) ? 4 : 0;
@@ -227,17 +237,18 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   uint32_t oa[4], ob[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    oa[s] = swz(wm * (MI * 32) + lr, 2 * s + lh);
-    ob[s] = TM * 128 + swz(wn * 64 + lr, 2 * s + lh);
+    const int c = 2 * (C::WK == 1 ? s : s ^ (2 * wk)) + lh;      // WK = 2: wave wk's two steps come first
+    oa[s] = swz(wm * (MI * 32) + lr, c);
+    ob[s] = TM * 128 + swz(wn * 64 + lr, c);
   }
   auto multiply = [&](f16v (&c)[MI][NI], uint32_t flip) BLK_INLINE {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int t = 0; t < 4 / C::WK; ++t) {
       i4v fa[MI], fb[NI];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) fb[j] = *(const i4v*)(lds + ((ob[s ^ (j & 1 ? 2 : 0)] + j * 4096) ^ flip));
+      for (int j = 0; j < NI; ++j) fb[j] = *(const i4v*)(lds + ((ob[t ^ (j & 1 ? 2 : 0)] + j * 4096) ^ flip));
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = *(const i4v*)(lds + ((oa[s ^ (i & 1 ? 2 : 0)] + i * 4096) ^ flip));
+      for (int i = 0; i < MI; ++i) fa[i] = *(const i4v*)(lds + ((oa[t ^ (i & 1 ? 2 : 0)] + i * 4096) ^ flip));
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -246,70 +257,93 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   };
 
   const int64_t ib = P.nb * split / P.splits, ie = P.nb * (split + 1) / P.splits;
-  uint32_t flip = HALF;                                  // the buffer being multiplied
+  // block i into registers
+  auto fetch = [&](int64_t i, typename decltype(sa)::Regs& va, typename decltype(sb)::Regs& vb) BLK_INLINE {
+    int64_t nk = 0;
+    if (run == 0) {                                      // a segment's first block, or one of its last
+      const int seg = i >= nb0;
+      const int64_t j = i - (seg ? nb0 : 0), k = j * BK, K = seg ? K1 : K0;
+      if (seg != cur) {
+        cur = seg;
+        la = seg ? lda1 : lda0;
+        lb = seg ? ldb1 : ldb0;
+        // rows behind an operand's last: the last one again, not stored
+        if constexpr (TA) sa.aim_cols(la, M - m0);
+        else sa.aim_rows([&](int r) BLK_INLINE { const int64_t left = M - 1 - m0; return (r < left ? r : left) * la; });
+        if constexpr (TB) sb.aim_cols(lb, N - n0);
+        else if constexpr (EPI == E_GATE)
+          sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; const int c = (r >> 6) * 32 + (r & 31); return (c < left ? c : left) * (r & 32 ? ldb1 : ldb0); });
+        else
+          sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; return (r < left ? r : left) * lb; });
+      }
+      pa = (const T*)(seg ? P.A[1] : P.A[0]) + (TA ? k * la + m0 : m0 * la + k);
+      pb = (const T*)(seg ? P.B[1] : P.B[0]) + (TB ? k * lb + n0 : n0 * lb + k);
+      if constexpr (EPI == E_GATE) pb1 = (const T*)P.B[1] + n0 * ldb1 + k;
+      run = K - spare > 0 ? (K - spare) / BK - j : 0;
+      if (run <= 0) {
+        run = 0;
+        nk = K - k;
+      }
+    }
+    if (run > 0) {
+      sa.load(va, pa, pa, 0, la);
+      sb.load(vb, pb, pb1, other, lb);
+      pa += TA ? BK * la : BK;
+      pb += TB ? BK * lb : BK;
+      if constexpr (EPI == E_GATE) pb1 += BK;
+      --run;
+    } else {
+      sa.load_guard(va, pa, pa, 0, la, nk, M - m0);
+      sb.load_guard(vb, pb, pb1, other, lb, nk, N - n0);
+    }
+  };
   const bool colsum = FORM == F_TN && P.colsum && tni == 0;
-  float cs[4] = {0.f, 0.f, 0.f, 0.f};
+  float cs[sa.NC] = {};
+  auto keep = [&](typename decltype(sa)::Regs& va, typename decltype(sb)::Regs& vb, uint32_t flip) BLK_INLINE {
+    if constexpr (FORM == F_TN)
+      if (colsum) sa.add_cols(va, cs);
+    sa.store(va, lds, flip);
+    sb.store(vb, lds, flip);
+  };
+  constexpr int DEPTH = TWO ? 1 : C::DEPTH;              // (two sets of sums leave no room)
+  typename decltype(sa)::Regs ra[DEPTH];
+  typename decltype(sb)::Regs rb[DEPTH];
+  // block i is multiplied from one buffer while block i + 1 goes from registers to the other and block i + DEPTH is on its way to registers
+  if constexpr (DEPTH == 1) {
+    uint32_t flip = HALF;
 #pragma unroll
-  for (int h = 0; h < (TWO ? 2 : 1); ++h)
-    for (int64_t i = h ? nb0 : ib - 1; i < (TWO && !h ? nb0 : ie); ++i) {
-      // ---- block i + 1 into registers
-      const bool more = i + 1 < ie;
-      if (more) {
-        int64_t nk = 0;
-        if (run == 0) {                                  // a segment's first block, or one of its last
-          const int seg = i + 1 >= nb0;
-          const int64_t j = i + 1 - (seg ? nb0 : 0), k = j * BK, K = seg ? K1 : K0;
-          if (seg != cur) {
-            cur = seg;
-            la = seg ? lda1 : lda0;
-            lb = seg ? ldb1 : ldb0;
-            // rows behind an operand's last: the last one again, not stored
-            if constexpr (TA) sa.aim_cols(la, M - m0);
-            else sa.aim_rows([&](int r) BLK_INLINE { const int64_t left = M - 1 - m0; return (r < left ? r : left) * la; });
-            if constexpr (TB) sb.aim_cols(lb, N - n0);
-            else if constexpr (EPI == E_GATE)
-              sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; const int c = (r >> 6) * 32 + (r & 31); return (c < left ? c : left) * (r & 32 ? ldb1 : ldb0); });
-            else
-              sb.aim_rows([&](int r) BLK_INLINE { const int64_t left = N - 1 - n0; return (r < left ? r : left) * lb; });
-          }
-          pa = (const T*)(seg ? P.A[1] : P.A[0]) + (TA ? k * la + m0 : m0 * la + k);
-          pb = (const T*)(seg ? P.B[1] : P.B[0]) + (TB ? k * lb + n0 : n0 * lb + k);
-          if constexpr (EPI == E_GATE) pb1 = (const T*)P.B[1] + n0 * ldb1 + k;
-          run = K - spare > 0 ? (K - spare) / BK - j : 0;
-          if (run <= 0) {
-            run = 0;
-            nk = K - k;
-          }
-        }
-        if (run > 0) {
-          sa.load(pa, pa, 0, la);
-          sb.load(pb, pb1, other, lb);
-          pa += TA ? BK * la : BK;
-          pb += TB ? BK * lb : BK;
-          if constexpr (EPI == E_GATE) pb1 += BK;
-          --run;
-        } else {
-          sa.load_guard(pa, pa, 0, la, nk, M - m0);
-          sb.load_guard(pb, pb1, other, lb, nk, N - n0);
-        }
+    for (int h = 0; h < (TWO ? 2 : 1); ++h)
+      for (int64_t i = h ? nb0 : ib - 1; i < (TWO && !h ? nb0 : ie); ++i) {
+        const bool more = i + 1 < ie;
+        if (more) fetch(i + 1, ra[0], rb[0]);
+        if (h || i >= ib) multiply(acc[TWO ? h : 0], flip);
+        flip ^= HALF;
+        if (more) keep(ra[0], rb[0], flip);
+        __syncthreads();
       }
-      if (h || i >= ib) multiply(acc[TWO ? h : 0], flip);
-      flip ^= HALF;
-      if (more) {
-        if constexpr (FORM == F_TN)
-          if (colsum) sa.add_cols(cs);
-        sa.store(lds, flip);
-        sb.store(lds, flip);
+  } else {
+    for (int64_t i = ib - 2; i < ie; i += 2) {
+      if (i + 2 < ie) fetch(i + 2, ra[0], rb[0]);
+      if (i >= ib) {
+        multiply(acc[0], 0);
+        if (i + 1 < ie) keep(ra[1], rb[1], HALF);
+        __syncthreads();
       }
+      if (i + 1 >= ie) break;
+      if (i + 3 < ie) fetch(i + 3, ra[1], rb[1]);
+      if (i >= ib) multiply(acc[0], HALF);
+      if (i + 2 < ie) keep(ra[0], rb[0], 0);
       __syncthreads();
     }
+    __syncthreads();
+  }
 
   // ---- column sums of A (a bias's gradient: the values are in hand, one column of tiles adds them up)
   if constexpr (FORM == F_TN) {
     if (colsum) {
       float* f = (float*)lds;                            // [8][TM]
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[sa.chunk() * TM + sa.col() + j] = cs[j];
+      for (int j = 0; j < sa.NC; ++j) f[sa.chunk() * TM + sa.col() + j] = cs[j];
       __syncthreads();
       for (int c = threadIdx.x; c < TM; c += NT)
         if (m0 + c < M) {
@@ -324,9 +358,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   }
 
   // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows
-  constexpr int PITCH = 68;                              // floats: 272 bytes, so that 8 rows' 16-byte pieces lie in different banks
   float* st = (float*)lds + wave * (32 * PITCH);
-  static_assert(sizeof(lds) >= (size_t)(NT / 64) * 32 * PITCH * 4, "epilogue staging");
   constexpr bool PAIR = EPI == E_GATE || EPI == E_GATE2;
   const int act = P.act;
 #pragma unroll
@@ -341,23 +373,34 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
           f4 v = {c[r4 * 4], c[r4 * 4 + 1], c[r4 * 4 + 2], c[r4 * 4 + 3]};
           *(f4*)(st + lr * PITCH + j * 32 + r4 * 8 + lh * 4) = v;
         }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      if constexpr (C::WK == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      } else {
+        __syncthreads();                                 // the sums of the waves that share the steps are added as they are read
+      }
       constexpr int LPR = PAIR ? 4 : 8;                  // lanes per row
 #pragma unroll 1
-      for (int p = 0; p < 32 * LPR / 64; ++p) {
+      for (int p = wk; p < 32 * LPR / 64; p += C::WK) {
         const int rr = p * (64 / LPR) + lane / LPR, nc = lane % LPR * 8;
         const int64_t m = m0 + wm * (MI * 32) + i * 32 + rr;
         const int64_t n = n0 + (EPI == E_GATE ? wn * 32 : EPI == E_GATE2 ? wn * 64 + q * 32 : wn * 64) + nc;
         if (m >= M || n >= N) continue;
         const int nv = N - n < 8 ? (int)(N - n) : 8;
         float v[8], u[8];
-        *(f4*)&v[0] = *(const f4*)(st + rr * PITCH + nc);
-        *(f4*)&v[4] = *(const f4*)(st + rr * PITCH + nc + 4);
-        if constexpr (PAIR) {
-          *(f4*)&u[0] = *(const f4*)(st + rr * PITCH + 32 + nc);
-          *(f4*)&u[4] = *(const f4*)(st + rr * PITCH + 32 + nc + 4);
-        }
+        auto sums = [&](float (&o)[8], int at) BLK_INLINE {
+          const float* q = st - wk * (32 * PITCH) + rr * PITCH + at;
+          f4 x = *(const f4*)q, y = *(const f4*)(q + 4);
+#pragma unroll
+          for (int k = 1; k < C::WK; ++k) {
+            x += *(const f4*)(q + k * (32 * PITCH));
+            y += *(const f4*)(q + k * (32 * PITCH) + 4);
+          }
+          *(f4*)&o[0] = x;
+          *(f4*)&o[4] = y;
+        };
+        sums(v, nc);
+        if constexpr (PAIR) sums(u, 32 + nc);
         if constexpr (EPI == E_DACT) {
           if (P.mask) {
             float h[8];
@@ -411,8 +454,12 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
           store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
         }
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      if constexpr (C::WK == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      } else {
+        __syncthreads();
+      }
     }
 }
 
@@ -579,14 +626,18 @@ template <int FORM, int EPI, int KIND> int go(const GemmArgs& a, int64_t tiles, 
 int BLK_ENTRY(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s) {
   if (tiles == 0) return DPVO_OK;
   if (kind == T_FEW) return epi == E_LIN ? few<E_LIN>(a, tiles, s) : epi == E_GATE ? few<E_GATE>(a, tiles, s) : few<E_GATE2>(a, tiles, s);
-#define BLK_GO(F, E) if (form == F && epi == E) return kind == T_BIG ? go<F, E, T_BIG>(a, tiles, s) : kind == T_SMALL ? go<F, E, T_SMALL>(a, tiles, s) : go<F, E, T_TILE>(a, tiles, s);
+#define BLK_GO(F, E) if (form == F && epi == E) switch (kind) { \
+    case T_BIG: return E == E_GATE2 ? DPVO_E_UNSUPPORTED : go<F, E, E == E_GATE2 ? T_TILE : T_BIG>(a, tiles, s); \
+    case T_SMALL: return go<F, E, T_SMALL>(a, tiles, s); \
+    case T_TINY: return go<F, E, T_TINY>(a, tiles, s); \
+    default: return go<F, E, T_TILE>(a, tiles, s); }
   BLK_GO(F_NT, E_LIN)
   BLK_GO(F_NT, E_GATE)
+  BLK_GO(F_NT, E_GATE2)
   BLK_GO(F_NN, E_LIN)
   BLK_GO(F_NN, E_DACT)
   BLK_GO(F_TN, E_LIN)
 #undef BLK_GO
-  if (form == F_NT && epi == E_GATE2) return kind == T_SMALL ? go<F_NT, E_GATE2, T_SMALL>(a, tiles, s) : go<F_NT, E_GATE2, T_TILE>(a, tiles, s);
   return DPVO_E_UNSUPPORTED;
 }
 

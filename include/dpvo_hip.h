@@ -598,7 +598,8 @@ typedef struct {
   int64_t M, N, K, Kv;
   int32_t dtype, activation;
 } dpvo_gated_linear_t;
-int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* stream);
+size_t dpvo_gated_linear_workspace_bytes(const dpvo_gated_linear_t* p);   /* 0 with w_up, and wherever the sum is not cut into parts */
+int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* ws, size_t ws_bytes, void* stream);
 
 /* Gradients of the two sums from dy [M,N] (leading dimension lddy): d_gate = dy * up * act'(gate), d_up = dy * act(gate), both [M,N] with
  * leading dimension ldo in `dtype`; up == NULL (no product): d_gate = dy * act'(gate) alone.  gate, up: f32 contiguous, as saved. */
