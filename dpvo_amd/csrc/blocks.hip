@@ -229,7 +229,7 @@ int norm_check(const dpvo_residual_norm_t* p) {
   if (!act_ok(p->gate_activation)) return DPVO_E_INVALID;
   if (p->gate_activation > DPVO_ACT_SILU) return DPVO_E_UNSUPPORTED;
   if (p->D > NORM_MAX_D || p->M > INT_MAX) return DPVO_E_UNSUPPORTED;
-  if (p->gate && (p->groups < 1 || p->M % p->groups || !p->f)) return DPVO_E_INVALID;
+  if (p->gate && p->M && (!p->f || p->groups < 1 || p->M % p->groups)) return DPVO_E_INVALID;
   if (p->M && !p->x) return DPVO_E_INVALID;
   return DPVO_OK;
 }

@@ -1,0 +1,209 @@
+"""dpvo_amd.blocks on the host: what each operator refuses, the C entries' argument checks, and the ctypes mirrors of their structs.  (No GPU.)"""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from dpvo_amd import _lib as L
+from dpvo_amd import blocks
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+z = torch.zeros
+H, D = torch.float16, torch.float64
+
+
+@pytest.mark.parametrize("call,why", [
+    (lambda: blocks.linear(z(3, 4), z(5, 3)), "its input has 4 features"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4, 1)), "its input has 4 features"),
+    (lambda: blocks.linear(z(()), z(5, 4)), "no feature dimension"),
+    (lambda: blocks.linear(z(3, 0), z(5, 0)), "no features"),
+    (lambda: blocks.linear(z(3, 4), z(0, 4)), "no features"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4), z(4)), "bias of weight"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4, dtype=H)), "must have the input's dtype"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4), z(5, dtype=H)), "must have the input's dtype"),
+    (lambda: blocks.linear(z(3, 4, dtype=D), z(5, 4, dtype=D)), "unsupported dtype"),
+    (lambda: blocks.linear(z(3, 4, dtype=torch.int32), z(5, 4, dtype=torch.int32)), "unsupported dtype"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4), activation="tanh"), "activation is 'tanh'"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4), activation=None), "activation is None"),
+    (lambda: blocks.linear(z(3, 4), z(5, 4, device="meta")), "tensors on cpu and meta"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(6, 4)), "w_gate makes 5 features, w_up 6"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), up_input=z(2, 4)), "up_input"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), up_input=z(1, 3, 4)), "up_input"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), up_input=z(3, 7)), "its input has 7 features"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), up_input=z(3, 4, dtype=H)), "up_input"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), residual=z(3, 4)), "residual"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), residual=z(5)), "residual"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), residual=z(3, 5, dtype=H)), "residual"),
+    (lambda: blocks.gated_feed_forward(z(3, 4), z(5, 4), z(5, 4), z(4, 6)), "its input has 5 features"),
+    (lambda: blocks.gated_feed_forward(z(3, 4), z(5, 4), z(5, 4), z(4, 5), b_down=z(5)), "bias of w_down"),
+    (lambda: blocks.gated_residual(z(3, 4), z(5, 4), None, z(6, 4), None, z(4, 6), None), "must make x's 4 features"),
+    (lambda: blocks.gated_residual(z(3, 4), z(4, 4), None, z(6, 4), None, z(5, 6), None), "must make x's 4 features"),
+    (lambda: blocks.gated_residual(z(3, 4), z(4, 4), None, z(6, 4), None, z(4, 5), None), "its input has 6 features"),
+    (lambda: blocks.norm(z(3, 4), z(5)), "weight is (5,)"),
+    (lambda: blocks.norm(z(3, 4), z(4), z(4, dtype=H)), "all of one dtype"),
+    (lambda: blocks.norm(z(3, 4), z(4, dtype=D)), "parameters are"),
+    (lambda: blocks.norm(z(3, 0)), "rows of 0 elements"),
+    (lambda: blocks.norm(z(1, 16385)), "rows of 16385 elements"),
+    (lambda: blocks.norm(z(3, 4), kind="batch"), "kind is 'batch'"),
+    (lambda: blocks.norm(z(3, 4), kind=None), "kind is None"),
+    (lambda: blocks.norm(z(3, 4, dtype=H), out_dtype=torch.float32), "out_dtype"),
+    (lambda: blocks.norm(z(3, 4), out_dtype=D), "out_dtype"),
+    (lambda: blocks.residual_norm(z(3, 4), z(2, 4)), "branch"),
+    (lambda: blocks.residual_norm(z(3, 4, dtype=H), z(3, 4)), "branch"),
+    (lambda: blocks.residual_norm(z(3, 4, dtype=H), z(3, 4, dtype=torch.bfloat16)), "branch"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), gate=z(2, 4)), "gate (2, 4) must be shaped"),
+    (lambda: blocks.residual_norm(z(2, 3, 4), z(2, 3, 4), gate=z(3, 4)), "must be shaped"),
+    (lambda: blocks.residual_norm(z(2, 3, 4), z(2, 3, 4), gate=z(1, 3, 4)), "must be shaped"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), gate=z(3, 1)), "does not go with x"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), gate=z(1, 3, 4)), "does not go with x"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), gate=z(3, 4, dtype=H)), "gate is torch.float16"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), gate=z(4), gate_activation="gelu"), "gate_activation is 'gelu'"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), z(4), norm=None), "without a norm"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), post_weight=z(4)), "without a post_norm"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4), z(4), post_norm="rms", post_weight=z(4, dtype=H)), "all of one dtype"),
+    (lambda: blocks.residual_norm(z(3, 4), z(3, 4, dtype=H), out_dtype=torch.bfloat16), "out_dtype"),
+    # right in every other respect: there is no CPU path
+    (lambda: blocks.linear(z(3, 4), z(5, 4), z(5)), "run on the GPU only"),
+    (lambda: blocks.gated_linear(z(3, 4), z(5, 4), z(5, 4), residual=z(3, 5)), "run on the GPU only"),
+    (lambda: blocks.gated_feed_forward(z(3, 4), z(5, 4), z(5, 4), z(4, 5)), "run on the GPU only"),
+    (lambda: blocks.gated_residual(z(3, 4), z(4, 4), None, z(6, 4), z(6), z(4, 6), None), "run on the GPU only"),
+    (lambda: blocks.norm(z(3, 4), z(4), z(4)), "run on the GPU only"),
+    (lambda: blocks.residual_norm(z(2, 3, 4), z(2, 3, 4), z(4), gate=z(2, 1, 4)), "run on the GPU only"),
+])
+def test_refusals(call, why):
+    with pytest.raises(L.DPVOHipError, match=None) as e:
+        call()
+    assert why in str(e.value), str(e.value)
+
+
+def test_rows_and_gate_rows():
+    """the leading dimension that a view is handed on with, and how many gate rows a shape stands for"""
+    t = z(6, 5, 8)
+    assert blocks._rows(t)[1] == 8 and blocks._rows(t)[0].shape == (30, 8)
+    v = z(10, 12)[:, :8]
+    assert blocks._rows(v)[1] == 12 and blocks._rows(v)[0].data_ptr() == v.data_ptr()
+    assert blocks._rows(z(8, 10).t())[1] == 8                                  # elements apart: copied
+    assert blocks._rows(z(1, 8).expand(4, 8))[1] == 8                          # rows on top of each other: copied
+    assert blocks._rows(z(8))[0].shape == (1, 8)
+    assert blocks._rows(z(0, 3, 8))[0].shape == (0, 8)
+    big = torch.empty(2, 5_000_000, dtype=H)[:, :8]
+    assert blocks._rows(big)[1] == 8                                           # too far apart for 32-bit offsets in a tile: copied
+    g = lambda x, s: blocks._gate_rows("t", z(*x), z(*s))  # noqa: E731
+    assert g((2, 3, 4), (4,)) == g((2, 3, 4), (1, 4)) == g((2, 3, 4), (1, 1, 4)) == 1
+    assert g((2, 3, 4), (2, 1, 4)) == 2 and g((2, 3, 4), (2, 3, 4)) == 6 and g((1, 3, 4), (3, 4)) == 3 and g((0, 4), (0, 4)) == 0
+
+
+def test_entries_check_their_arguments():
+    """error codes before anything touches the device"""
+    lib, null, INVALID, UNSUPPORTED, WORKSPACE = L.lib(), None, -1, -2, -3
+    one = ctypes.addressof(ctypes.c_int64(0))                                   # an address that no accepted call reads
+    p = L.GatedLinear()
+    assert lib.dpvo_gated_linear(null, null, 0, null) == INVALID and lib.dpvo_gated_linear_workspace_bytes(null) == 0
+    assert lib.dpvo_gated_linear(ctypes.byref(p), null, 0, null) == 0           # no rows: nothing to do
+    ok = dict(x=one, w_gate=one, y=one, ldx=64, ldwg=64, ldy=32, M=70, N=32, K=64, dtype=0)
+
+    def call(**kw):
+        q = L.GatedLinear()
+        for k, v in {**ok, **kw}.items():
+            setattr(q, k, v)
+        return lib.dpvo_gated_linear(ctypes.byref(q), null, 0, null)
+    for bad in (dict(M=-1), dict(N=-1), dict(K=-1), dict(Kv=-1), dict(dtype=3), dict(activation=6), dict(activation=-1), dict(x=None), dict(y=None),
+                dict(w_gate=None), dict(ldx=63), dict(ldwg=63), dict(ldy=31), dict(residual=one, ldr=31), dict(w_up=one, Kv=8, ldv=8, ldwu=8, v=None),
+                dict(w_up=one, v=one, Kv=8, ldv=7, ldwu=8), dict(w_up=one, v=one, Kv=8, ldv=8, ldwu=7), dict(ldx=2 ** 31)):
+        assert call(**bad) == INVALID, bad
+    q = L.GatedLinear()
+    for k, v in {**ok, "M": 100, "N": 64, "K": 64 * 64, "ldx": 64 * 64, "ldwg": 64 * 64, "ldy": 64}.items():
+        setattr(q, k, v)
+    assert lib.dpvo_gated_linear_workspace_bytes(ctypes.byref(q)) > 0 and lib.dpvo_gated_linear(ctypes.byref(q), null, 0, null) == WORKSPACE
+    assert lib.dpvo_gated_linear_dact(null, 4, null, null, null, null, 4, 0, 0, 3, 4, null) == INVALID
+    assert lib.dpvo_gated_linear_dact(null, 4, null, null, null, null, 4, 0, 0, 0, 4, null) == 0
+    assert lib.dpvo_gated_linear_dact(one, 4, one, one, one, null, 4, 0, 3, 3, 4, null) == INVALID
+    assert lib.dpvo_gated_linear_dact(one, 3, one, null, one, null, 4, 0, 3, 3, 4, null) == INVALID
+
+    def dx(**kw):
+        q = L.GatedLinearDx()
+        q.a[0] = q.b[0] = q.dx = one
+        q.lda[0], q.ldb[0], q.K[0], q.lddx, q.M, q.N = 64, 32, 64, 32, 70, 32
+        for k, v in kw.items():
+            if isinstance(v, tuple):
+                getattr(q, k)[v[0]] = v[1]
+            else:
+                setattr(q, k, v)
+        return q, lib.dpvo_gated_linear_dx(ctypes.byref(q), null, 0, null)
+    assert lib.dpvo_gated_linear_dx(null, null, 0, null) == INVALID and lib.dpvo_gated_linear_dx_workspace_bytes(null) == 0
+    for bad in (dict(M=-1), dict(N=-2), dict(K=(0, -1)), dict(dtype=7), dict(activation=9), dict(a=(0, None)), dict(b=(0, None)), dict(dx=None), dict(lda=(0, 63)),
+                dict(ldb=(0, 31)), dict(lddx=31), dict(addend=one, ldadd=3), dict(mask=one, ldmask=3), dict(gate=one, mask=one, ldmask=32), dict(up=one),
+                dict(gate=one, up=one)):
+        assert dx(**bad)[1] == INVALID, bad
+    assert dx(gate=one, addend=one, ldadd=32)[1] == UNSUPPORTED
+    q, rc = dx(M=64, N=64, K=(0, 64 * 64), lda=(0, 64 * 64), ldb=(0, 64), lddx=64)
+    assert rc == WORKSPACE and lib.dpvo_gated_linear_dx_workspace_bytes(ctypes.byref(q)) >= 2 * 64 * 64 * 4
+
+    def dw(**kw):
+        q = L.GatedLinearDw()
+        q.a[0] = q.b[0] = q.dw[0] = one
+        q.lda[0], q.ldb[0], q.N[0], q.K[0], q.M, q.n = 32, 64, 32, 64, 70, 1
+        for k, v in kw.items():
+            if isinstance(v, tuple):
+                getattr(q, k)[v[0]] = v[1]
+            else:
+                setattr(q, k, v)
+        return lib.dpvo_gated_linear_dw(ctypes.byref(q), null, 0, null)
+    for bad in (dict(M=-1), dict(n=5), dict(n=-1), dict(dtype=3), dict(N=(0, -1)), dict(K=(0, -1)), dict(a=(0, None)), dict(b=(0, None)), dict(dw=(0, None)),
+                dict(lda=(0, 31)), dict(ldb=(0, 63))):
+        assert dw(**bad) == INVALID, bad
+    assert dw(n=0) == 0 and dw(M=45312) == WORKSPACE
+
+    def rn(back=False, **kw):
+        q = L.ResidualNorm()
+        q.x = q.f = q.s = q.h = one
+        q.ldx = q.ldf = q.D = 32
+        q.M, q.groups, q.x_dtype, q.f_dtype, q.h_dtype, q.w_dtype, q.norm, q.scale = 5, 5, 1, 1, 1, 1, 1, 1.0
+        for k, v in kw.items():
+            setattr(q, k, v)
+        return lib.dpvo_residual_norm_backward(ctypes.byref(q), null, 0, null) if back else lib.dpvo_residual_norm(ctypes.byref(q), null)
+    assert lib.dpvo_residual_norm(null, null) == INVALID and lib.dpvo_residual_norm_backward(null, null, 0, null) == INVALID
+    for bad in (dict(M=-1), dict(D=0), dict(x_dtype=3), dict(f_dtype=-1), dict(w_dtype=9), dict(norm=3), dict(post=-1), dict(gate_activation=7), dict(x=None),
+                dict(gate=one, ldgate=32, groups=0), dict(gate=one, ldgate=32, groups=2), dict(gate=one, ldgate=31), dict(ldx=31), dict(ldf=31), dict(h=None),
+                dict(norm=0, s=None), dict(gate=one, ldgate=32, f=None)):
+        assert rn(**bad) == INVALID, bad
+    for bad in (dict(x_dtype=0), dict(h_dtype=2), dict(D=16385, ldx=16385, ldf=16385), dict(gate_activation=4), dict(M=2 ** 31)):
+        assert rn(**bad) == UNSUPPORTED, bad
+    assert rn(M=0) == 0
+    for bad in (dict(ds=one, ldds=3), dict(dh=one, lddh=3), dict(dgate=one), dict(f=None, df=one), dict(dpw=one)):
+        assert rn(True, **bad) == INVALID, bad
+    assert rn(True, dh=one, lddh=32, dw=one) == WORKSPACE
+    assert rn(True, M=0) == 0
+
+
+def test_structs_match_the_header(tmp_path):
+    probes = {"dpvo_gated_linear_t": L.GatedLinear, "dpvo_gated_linear_dx_t": L.GatedLinearDx, "dpvo_gated_linear_dw_t": L.GatedLinearDw,
+              "dpvo_residual_norm_t": L.ResidualNorm}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "dpvo_hip.h"', 'int main(void) {']
+    for c, cls in probes.items():
+        lines.append(f'  printf("{c} %zu\\n", sizeof({c}));')
+        lines += [f'  printf("{c}.{f} %zu\\n", offsetof({c}, {f}));' for f, _ in cls._fields_]
+    src = tmp_path / "probe.c"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "probe")])
+    out = dict(l.split() for l in subprocess.check_output([str(tmp_path / "probe")], text=True).splitlines())
+    for c, cls in probes.items():
+        assert int(out[c]) == ctypes.sizeof(cls), c
+        for f, _ in cls._fields_:
+            assert int(out[f"{c}.{f}"]) == getattr(cls, f).offset, (c, f)
+    hdr = open(os.path.join(ROOT, "include", "dpvo_hip.h")).read()
+    import re
+    codes = {k: int(v) for k, v in re.findall(r"#define DPVO_((?:ACT|NORM)_[A-Z_]+|F16|F32|BF16) (\d+)", hdr)}
+    assert {k: codes["ACT_" + k.upper()] for k in blocks.ACTIVATIONS} == blocks.ACTIVATIONS
+    assert {"layer": codes["NORM_LAYER"], "rms": codes["NORM_RMS"], None: codes["NORM_NONE"]} == blocks.NORMS
+    assert (codes["F16"], codes["F32"], codes["BF16"]) == (L.F16, L.F32, L.BF16)
+
+
+def test_state_dict_keys_stay():
+    """the stage that became callable keeps its names in a checkpoint"""
+    from dpvo_amd import net as N
+    keys = list(N.Update(3).gru.state_dict())
+    assert keys == ["0.weight", "0.bias"] + [f"1.{k}.{w}" for k in ("gate.0", "res.0", "res.2") for w in ("weight", "bias")] + ["2.weight", "2.bias"] + \
+        [f"3.{k}.{w}" for k in ("gate.0", "res.0", "res.2") for w in ("weight", "bias")]

@@ -59,6 +59,11 @@ def rows_f(x):
     return V(x.detach().double().cpu())
 
 
+def on_gpu(x):
+    """the same on the GPU, for sizes where the CPU's 64-bit products would take long"""
+    return V(x.detach().double())
+
+
 def act(name, z):
     """(value, derivative) with the bounds of both.  Each function and its derivative has a slope of at most 1.2; the hardware exponential
     is good to |z| 2^-23 + 2^-22 relative, what it makes is at most about |z| + 1."""
@@ -89,7 +94,7 @@ def proj(x, w, b=None):
 
 def within(got, want, t, what):
     want = want.to(t)
-    g = got.detach().double().cpu().reshape(want.v.shape)
+    g = got.detach().double().to(want.v.device).reshape(want.v.shape)
     assert got.dtype == t, (what, got.dtype)
     bad = ~((g - want.v).abs() <= want.e)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside their bound; worst error "
@@ -394,6 +399,339 @@ def residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, us
 def test_residual_norm(dev, tx, tb, lead, D, kind, post, gate, gate_act, scale, use):
     g = torch.Generator().manual_seed(D + len(lead))
     residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, use)
+
+
+# ------------------------------------------------------------------------------------------------------------------ large tiles and long sums
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,F,N", [(5013, 2311, 2317, 2305), (4100, 1030, 2310, 1030), (20011, 200, 136, 72), (45312, 384, 384, 384), (2000, 1500, 700, 300)])
+def test_feed_forward_large(dev, t, M, K, F, N):
+    """sizes that reach the 256- and 128-wide tiles of every product, sums in parts, and tiles that hang over in both directions"""
+    g = torch.Generator().manual_seed(M)
+    x = make(g, M, K, t=t)
+    wg, bg = layer(g, F, K, t)
+    wu, bu = layer(g, F, K, t)
+    wd, bd = layer(g, N, F, t)
+    dy = make(g, M, N, t=t, grad=False)
+    f = on_gpu
+    h, G, Uu, ya, da = gated_reference(f(x), f(wg), f(wu), f(bg), f(bu), "silu")
+    h = h.to(t)
+    y = blocks.gated_feed_forward(x, wg, wu, wd, bg, bu, bd, "silu")
+    within(y, proj(h, f(wd), f(bd)), t, "y")
+    grads = torch.autograd.grad(y, [x, wg, wu, wd, bg, bu, bd], dy)
+    D = f(dy)
+    dh = D.mm(f(wd))
+    dg, du = (dh * Uu * da).to(t), (dh * ya).to(t)
+    want = [dg.mm(f(wg)) + du.mm(f(wu)), dg.t().mm(f(x)), du.t().mm(f(x)), D.t().mm(h), dg.sum0(), du.sum0(), D.sum0()]
+    for name, got, w in zip(("dx", "dwg", "dwu", "dwd", "dbg", "dbu", "dbd"), grads, want):
+        within(got, w, t, name)
+    again = torch.autograd.grad(blocks.gated_feed_forward(x, wg, wu, wd, bg, bu, bd, "silu"), [x, wg, wu, wd, bg, bu, bd], dy)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))       # no order of sums changes from run to run
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N", [(5013, 2311, 2317), (9000, 384, 390)])
+def test_gated_linear_large_two_inputs(dev, t, M, K, N):
+    g = torch.Generator().manual_seed(M + 1)
+    x, v, res = make(g, M, K, t=t), make(g, M, K + 5, t=t), make(g, M, N, t=t)
+    wg, bg = layer(g, N, K, t)
+    wu, bu = layer(g, N, K + 5, t)
+    dy = make(g, M, N, t=t, grad=False)
+    f = on_gpu
+    y = blocks.gated_linear(x, wg, wu, bg, bu, "sigmoid", up_input=v, residual=res)
+    out, G, Uu, ya, da = gated_reference(f(x), f(wg), f(wu), f(bg), f(bu), "sigmoid", f(v), f(res))
+    within(y, out, t, "y")
+    grads = torch.autograd.grad(y, [x, v, wg, wu, bg, bu], dy)
+    D = f(dy)
+    dg, du = (D * Uu * da).to(t), (D * ya).to(t)
+    want = [dg.mm(f(wg)), du.mm(f(wu)), dg.t().mm(f(x)), du.t().mm(f(v)), dg.sum0(), du.sum0()]
+    for name, got, w in zip(("dx", "dv", "dwg", "dwu", "dbg", "dbu"), grads, want):
+        within(got, w, t, name)
+
+
+# ------------------------------------------------------------------------------------------------------------------ layouts
+def odd_place(x, ld=None, shift=1):
+    """the same values at an address `shift` elements behind an allocation's, with rows `ld` apart"""
+    M, K = x.shape
+    ld = ld or K
+    buf = torch.full((shift + M * ld + 7,), float("nan"), dtype=x.dtype, device=x.device)
+    v = buf[shift:shift + M * ld].view(M, ld)[:, :K]
+    v.copy_(x)
+    return v
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N", [(5, 33, 17), (70, 129, 65), (300, 384, 200), (1100, 250, 390)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_unaligned_rows(dev, t, M, K, N, pad):
+    """rows that start at any element, with NaN between and behind them: nothing outside a row may be used"""
+    g = torch.Generator().manual_seed(M + pad)
+    x, wg, wu = make(g, M, K, t=t, grad=False), make(g, N, K, t=t, scale=0.1, grad=False), make(g, N, K, t=t, scale=0.1, grad=False)
+    b, res, dy = make(g, N, t=t, grad=False), make(g, M, N, t=t, grad=False), make(g, M, N, t=t, grad=False)
+    for a in ("silu", "identity"):
+        want = [p.clone().requires_grad_() for p in (x, wg, wu, b, res)]
+        y0 = blocks.gated_linear(want[0], want[1], want[2], want[3], want[3], a, residual=want[4])
+        g0 = torch.autograd.grad(y0, want, dy)
+        got = [odd_place(p, p.shape[1] + pad).requires_grad_() for p in (x, wg, wu)] + [odd_place(b[None])[0].requires_grad_(),
+                                                                                      odd_place(res, N + pad).requires_grad_()]
+        y1 = blocks.gated_linear(got[0], got[1], got[2], got[3], got[3], a, residual=got[4])
+        g1 = torch.autograd.grad(y1, got, odd_place(dy, N + pad))
+        assert torch.equal(y0, y1)
+        assert all(torch.equal(p, q) for p, q in zip(g0, g1))
+    for p, q in ((x, odd_place(x, K + pad)), (x.t().contiguous().t(), x.t().contiguous().t())):
+        assert torch.equal(blocks.linear(x, wg, b), blocks.linear(q, odd_place(wg, K + pad), b))
+    w = make(g, K, t=t, grad=False)
+    assert torch.equal(blocks.norm(x, w), blocks.norm(odd_place(x, K + pad), odd_place(w[None])[0]))
+    s0 = blocks.residual_norm(x, x, w, gate=w, post_norm="rms", post_weight=w)
+    s1 = blocks.residual_norm(odd_place(x, K + pad), odd_place(x, K + pad, 3), odd_place(w[None])[0], gate=odd_place(w[None])[0], post_norm="rms", post_weight=w)
+    assert all(torch.equal(p, q) for p, q in zip(s0, s1))
+
+
+def test_layouts_are_accepted(dev):
+    """any strides, leading shapes and broadcast gradients give what contiguous rows give"""
+    g = torch.Generator().manual_seed(0)
+    x = make(g, 6, 5, 24, grad=False)
+    w, wu = make(g, 10, 24, scale=0.2, grad=False), make(g, 10, 24, scale=0.2, grad=False)
+    flat = blocks.gated_linear(x.reshape(30, 24), w, wu)
+    assert torch.equal(blocks.gated_linear(x, w, wu).reshape(30, 10), flat)
+    assert torch.equal(blocks.gated_linear(x.transpose(0, 1), w, wu), blocks.gated_linear(x.transpose(0, 1).contiguous(), w, wu))
+    assert torch.equal(blocks.gated_linear(x, w.t().contiguous().t(), wu).reshape(30, 10), flat)
+    assert torch.equal(blocks.gated_linear(x[0, 0], w, wu), flat[0])              # a vector
+    assert torch.equal(blocks.gated_linear(x[:1, :1].expand(3, 4, 24), w, wu), flat[:1, None].expand(1, 12, 10).reshape(3, 4, 10))
+    p = x.clone().requires_grad_()
+    a, = torch.autograd.grad(blocks.gated_linear(p, w, wu).sum(), p)              # the gradient that arrives is an expanded scalar
+    b, = torch.autograd.grad(blocks.gated_linear(p, w, wu), p, torch.ones(6, 5, 10, device=dev))
+    assert torch.equal(a, b)
+    a, = torch.autograd.grad(blocks.norm(p).sum(), p)
+    b, = torch.autograd.grad(blocks.norm(p), p, torch.ones_like(x))
+    assert torch.equal(a, b)
+    same = [w.clone().requires_grad_()]                                           # one leaf in two places
+    got, = torch.autograd.grad(blocks.gated_linear(x, same[0], same[0]).sum(), same)
+    two = [w.clone().requires_grad_(), w.clone().requires_grad_()]
+    ga, gb = torch.autograd.grad(blocks.gated_linear(x, *two).sum(), two)
+    assert torch.equal(got, ga + gb)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_no_rows(dev, t):
+    x = torch.zeros(0, 3, 40, dtype=t, device=dev, requires_grad=True)
+    w, b = torch.ones(24, 40, dtype=t, device=dev, requires_grad=True), torch.ones(24, dtype=t, device=dev, requires_grad=True)
+    wd = torch.ones(40, 24, dtype=t, device=dev, requires_grad=True)
+    for y, leaves in ((blocks.linear(x, w, b, "relu"), [x, w, b]), (blocks.gated_linear(x, w, w, b, b), [x, w, b]),
+                      (blocks.gated_feed_forward(x, w, w, wd, b, b), [x, w, b, wd]), (blocks.norm(x, wd[:, 0], wd[:, 1]), [x, wd])):
+        assert y.shape[:2] == (0, 3)
+        for p, q in zip(leaves, torch.autograd.grad(y, leaves, torch.zeros_like(y))):
+            assert q.shape == p.shape and not q.any()
+    gate = torch.ones(0, 1, 40, dtype=t, device=dev, requires_grad=True)
+    row = torch.ones(40, dtype=t, device=dev, requires_grad=True)
+    for ga in (gate, row):
+        s, h = blocks.residual_norm(x, x, row, gate=ga)
+        assert s.shape == h.shape == x.shape
+        for p, q in zip((x, row, ga), torch.autograd.grad([s, h], [x, row, ga], [torch.zeros_like(s), torch.zeros_like(h)], allow_unused=True)):
+            assert q.shape == p.shape and not q.any()
+
+
+def test_some_gradients(dev):
+    """whatever subset of the leaves asks for a gradient, each gets what it gets when all ask"""
+    g = torch.Generator().manual_seed(2)
+    base = dict(x=make(g, 70, 48), wg=make(g, 36, 48), wu=make(g, 36, 48), wd=make(g, 48, 36), bg=make(g, 36), bu=make(g, 36), bd=make(g, 48))
+    run = {"ff": (lambda d: [blocks.gated_feed_forward(d["x"], d["wg"], d["wu"], d["wd"], d["bg"], d["bu"], d["bd"])], list(base)),
+           "block": (lambda d: [blocks.gated_residual(d["x"], d["sq"], d["bd"], d["wg"], d["bg"], d["wd"], d["bd"])], ["x", "wg", "wd", "bg", "sq"]),
+           "linear": (lambda d: [blocks.linear(d["x"], d["wg"], d["bg"], "silu")], ["x", "wg", "bg"]),
+           "two": (lambda d: [blocks.gated_linear(d["x"], d["wg"], d["sq"][:36, :36].contiguous(), d["bg"], d["bu"], up_input=d["v"], residual=d["v"])],
+                   ["x", "wg", "sq", "bg", "bu", "v"]),
+           "norm": (lambda d: list(blocks.residual_norm(d["x"], d["f"], d["n"], d["bd"], gate=d["gate"], gate_activation="sigmoid", post_norm="layer",
+                                                        post_weight=d["pn"], post_bias=d["pb"])), ["x", "f", "n", "bd", "gate", "pn", "pb"])}
+    base.update(sq=make(g, 48, 48), v=make(g, 70, 36), f=make(g, 70, 48), n=make(g, 48), gate=make(g, 48), pn=make(g, 48), pb=make(g, 48))
+    for name, (f, leaves) in run.items():
+        outs = f(base)
+        ups = [torch.randn(o.shape, generator=g).cuda() for o in outs]
+        full = dict(zip(leaves, torch.autograd.grad(outs, [base[k] for k in leaves], ups)))
+        for n in range(len(leaves)):
+            for some in ([leaves[n]], leaves[:n] + leaves[n + 1:]):
+                d = {k: v.detach().requires_grad_(k in some) for k, v in base.items()}
+                for k, got in zip(some, torch.autograd.grad(f(d), [d[k] for k in some], ups)):
+                    assert torch.equal(got, full[k]), (name, some, k)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_infinities_and_nan_stay_in_their_rows(dev, t):
+    g = torch.Generator().manual_seed(5)
+    for M, K, N in ((3, 70, 40), (100, 70, 40), (300, 200, 150)):
+        x, w, wu = make(g, M, K, t=t, grad=False), make(g, N, K, t=t, scale=0.1, grad=False), make(g, N, K, t=t, scale=0.1, grad=False)
+        y = blocks.gated_linear(x, w, wu)
+        bad = x.clone()
+        bad[1, 5], bad[2, 7] = float("nan"), float("inf")
+        z = blocks.gated_linear(bad, w, wu)
+        keep = [i for i in range(M) if i not in (1, 2)]
+        assert torch.equal(z[keep], y[keep]) and z[1].isnan().all() and not z[2].isfinite().all()
+        wb = w.clone()
+        wb[4, 3] = float("nan")                                       # one output column
+        z = blocks.gated_linear(x, wb, wu)
+        cols = [i for i in range(N) if i != 4]
+        assert torch.equal(z[:, cols], y[:, cols]) and z[:, 4].isnan().all()
+        n0, n1 = blocks.norm(x), blocks.norm(bad)
+        assert torch.equal(n1[keep], n0[keep]) and n1[1].isnan().all()
+        p, q = x.clone().requires_grad_(), w.clone().requires_grad_()
+        dy = make(g, M, N, t=t, grad=False)
+        d0 = torch.autograd.grad(blocks.gated_linear(p, q, wu), [p, q], dy)
+        db = dy.clone()
+        db[1, 6] = float("nan")
+        d1 = torch.autograd.grad(blocks.gated_linear(p, q, wu), [p, q], db)
+        assert torch.equal(d1[0][keep], d0[0][keep]) and d1[0][1].isnan().all()
+        cols = [i for i in range(N) if i != 6]
+        assert torch.equal(d1[1][cols], d0[1][cols]) and d1[1][6].isnan().all()
+
+
+def test_many_elements(dev):
+    """offsets that pass 32 bits: 36 million rows of 64 in 16 bits (2.3e9 elements), first and last rows against a small call"""
+    M, K, N = 36_000_000, 8, 64
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(M, K, generator=g, device=dev).half()
+    w, wu = torch.randn(N, K, generator=g, device=dev).half(), torch.randn(N, K, generator=g, device=dev).half()
+    y = blocks.gated_linear(x, w, wu)
+    for a, b in ((0, 5000), (M // 2 - 77, M // 2 + 4001), (M - 5000, M)):
+        assert torch.equal(y[a:b], blocks.gated_linear(x[a:b], w, wu))
+    s, h = blocks.residual_norm(y, y, norm="rms")
+    for a, b in ((0, 50), (M - 50, M)):
+        s1, h1 = blocks.residual_norm(y[a:b], y[a:b], norm="rms")
+        assert torch.equal(s[a:b], s1) and torch.equal(h[a:b], h1)
+    del s, h
+    # a weight's gradient over all of them: 1 in the rows that count, 0 elsewhere
+    p = w.clone().requires_grad_()
+    dy = torch.zeros_like(y)
+    dy[-3:] = 1
+    got, = torch.autograd.grad(blocks.linear(x, p), p, dy)
+    torch.testing.assert_close(got.float(), x[-3:].float().sum(0).expand(N, K), rtol=2.0 ** -11, atol=1e-6)
+
+
+# ------------------------------------------------------------------------------------------------------------------ streams and graphs
+def block_step(d):
+    """norm -> gated feed-forward -> (gate, residual) -> norm -> gated residual block, and all gradients"""
+    h = blocks.norm(d["x"], d["n1"], d["b1"])
+    f = blocks.gated_feed_forward(h, d["wg"], d["wu"], d["wd"], d["bg"], d["bg"], d["n1"])
+    s, h = blocks.residual_norm(d["x"], f, d["n2"], norm="rms", gate=d["gate"], gate_activation="sigmoid", scale=0.5, post_norm="layer", post_weight=d["n1"],
+                                post_bias=d["b1"])
+    y = blocks.gated_residual(h, d["sq"], d["b1"], d["wg"], d["bg"], d["wd"], d["b1"])
+    return [s, y, *torch.autograd.grad([s, y], list(d.values()), [torch.ones_like(s), torch.full_like(y, 0.5)])]
+
+
+def block_leaves(t, M=200, D=96, F=160, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return {"x": make(g, M, D, t=t), "n1": make(g, D, t=t, scale=0.2, mean=1.0), "b1": make(g, D, t=t, scale=0.2), "wg": make(g, F, D, t=t, scale=0.1),
+            "wu": make(g, F, D, t=t, scale=0.1), "wd": make(g, D, F, t=t, scale=0.1), "bg": make(g, F, t=t, scale=0.2), "n2": make(g, D, t=t, scale=0.2, mean=1.0),
+            "gate": make(g, D, t=t), "sq": make(g, D, D, t=t, scale=0.1)}
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_the_run_of_them_on_two_streams(dev, t):
+    """two runs at once on two streams give what each gives alone"""
+    a, b = block_leaves(t), block_leaves(t, M=333, seed=1)
+    want = [block_step(a), block_step(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for st, d in zip(streams, (a, b)):
+            with torch.cuda.stream(st):
+                got.append(block_step(d))
+        torch.cuda.synchronize()
+        for w, q in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(w, q))
+
+
+def test_captured_graphs(dev):
+    """two graphs of forward passes (with and without sums in parts) and one of a whole step, replayed in turn with eager calls between: every replay
+    equals the eager result on the inputs of the moment"""
+    leaves = {k: v.detach() for k, v in block_leaves(F16, M=200, D=384, F=2048).items()}
+
+    def forward(d):
+        h = blocks.norm(d["x"], d["n1"], d["b1"])
+        f = blocks.gated_feed_forward(h, d["wg"], d["wu"], d["wd"], d["bg"], d["bg"], d["n1"])
+        return list(blocks.residual_norm(d["x"], f, d["n2"], norm="rms", gate=d["gate"]))
+
+    def step(d):
+        return block_step({k: v.detach().requires_grad_() for k, v in d.items()})
+
+    wide = {"x": torch.randn(64, 4096, device=dev).half()}
+
+    def wide_step(d):
+        x = d["x"].detach().requires_grad_()
+        w, b = torch.ones(4096, device=dev).half().requires_grad_(), torch.ones(4096, device=dev).half().requires_grad_()
+        s, h = blocks.residual_norm(x, x * 0.5, w, b, gate=w, post_norm="layer", post_weight=w, post_bias=b)
+        return [h, *torch.autograd.grad([s, h], [x, w, b], [torch.ones_like(s), torch.ones_like(h)])]
+
+    jobs = []
+    for f, d in ((forward, leaves), (step, leaves), (forward, {**leaves, "x": leaves["x"][:50].clone()}), (wide_step, wide)):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            f(d)
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f(d)
+        jobs.append((f, d, graph, out))
+    for k in range(4):
+        for f, d, graph, out in jobs:
+            d["x"].copy_(torch.randn(d["x"].shape, generator=torch.Generator().manual_seed(k)).half())
+            graph.replay()
+            want = f(d)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, want)), (f.__name__, k)
+
+
+def test_second_order_is_refused(dev):
+    x = torch.randn(4, 8, device=dev, requires_grad=True)
+    w = torch.randn(8, 8, device=dev, requires_grad=True)
+    g, = torch.autograd.grad(blocks.linear(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), w)
+
+
+def test_gradients_against_differences(dev):
+    """the gradients of a whole run in f32 against central differences of the plain formula in 64 bits along random directions"""
+    d = block_leaves(F32, M=20, D=24, F=32)
+    grads = block_step(d)[2:]
+    g = torch.Generator().manual_seed(9)
+    val = {k: v.detach().double().cpu() for k, v in d.items()}
+    dirs = {k: torch.randn(v.shape, generator=g, dtype=torch.float64) for k, v in val.items()}
+
+    def loss(v):
+        ln = lambda x, w, b: torch.nn.functional.layer_norm(x, x.shape[-1:], w, b, 1e-3)  # noqa: E731
+        rms = lambda x, w: x * (x.pow(2).mean(-1, keepdim=True) + 1e-3).rsqrt() * w  # noqa: E731
+        lin = torch.nn.functional.linear
+        h = ln(v["x"], v["n1"], v["b1"])
+        f = lin(torch.nn.functional.silu(lin(h, v["wg"], v["bg"])) * lin(h, v["wu"], v["bg"]), v["wd"], v["n1"])
+        s = v["x"] + 0.5 * torch.sigmoid(v["gate"]) * ln(f, v["n1"], v["b1"])
+        h = rms(s, v["n2"])
+        y = h + torch.sigmoid(lin(h, v["sq"], v["b1"])) * lin(torch.relu(lin(h, v["wg"], v["bg"])), v["wd"], v["b1"])
+        return s.sum() + 0.5 * y.sum()
+
+    e = 1e-5
+    for k, got in zip(d, grads):
+        up, dn = dict(val), dict(val)
+        up[k], dn[k] = val[k] + e * dirs[k], val[k] - e * dirs[k]
+        want = float(loss(up) - loss(dn)) / (2 * e)
+        have = float((got.double().cpu() * dirs[k]).sum())
+        # f32 sums of some hundred terms, and e^2 of the difference
+        assert abs(have - want) < 2e-4 * float((got.double().cpu().abs() * dirs[k].abs()).sum()) + 1e-6, (k, have, want)
+
+
+def test_the_bounds_see_a_mistake():
+    """the oracle with a sign, a factor or a dropped term is outside the bounds by which the kernels are held (nothing runs on the GPU here)"""
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(40, 64, generator=g).half(), (torch.randn(30, 64, generator=g) / 8).half()
+    z = proj(rows_f(x), rows_f(w))
+    v, d = act("silu", z)
+    for wrong in (v.v * 1.002, v.v + 2e-3, torch.relu(z.v), v.v.roll(1, 0)):
+        with pytest.raises(AssertionError):
+            within(wrong.half(), v, F16, "planted")
+    within(v.v.half(), v, F16, "right")
+    xh, r = normalise(rows_f(x), "layer", 1e-3)
+    for wrong in (normalise(rows_f(x), "rms", 1e-3)[0].v, normalise(rows_f(x), "layer", 1e-2)[0].v):
+        with pytest.raises(AssertionError):
+            within(wrong.half(), xh, F16, "planted")
 
 
 # ------------------------------------------------------------------------------------------------------------------ together, as the model has them
