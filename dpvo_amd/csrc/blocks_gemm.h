@@ -361,14 +361,61 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
     }
   }
 
-  // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows
+  // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows.  Where there
+  // are two sums, or an activation, a rolled loop does the work (the activations are long); where there is one, what follows it is short and
+  // unrolled, and what that needs from memory (a residual, a mask) is requested for all its rows beforehand, so that a piece waits once
+  // (8192 x 8192 x 4096: 499 -> 488 us, 4096 x 4096 x 1024: 43.4 -> 39.0; the pairs gain nothing by it).
   float* st = (float*)lds + wave * (32 * PITCH);
+  float* const st0 = st - wk * (32 * PITCH);             // of the first of the waves that share the steps
   constexpr bool PAIR = EPI == E_GATE || EPI == E_GATE2;
+  constexpr int LPR = PAIR ? 4 : 8, RPP = 64 / LPR;      // lanes per row, rows per pass
+  constexpr int NP = 32 / RPP / C::WK;                   // passes of this wave
   const int act = P.act;
+  const bool parts = EPI == E_LIN && P.part;
+  const int nc = lane % LPR * 8;
+  // a pass's row of this lane; a row's sums
+  auto row_of = [&](int p) BLK_INLINE { return (p * C::WK + wk) * RPP + lane / LPR; };
+  auto sums = [&](float (&o)[8], int rr, int at) BLK_INLINE {
+    const float* q = st0 + rr * PITCH + at;
+    f4 x = *(const f4*)q, y = *(const f4*)(q + 4);
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+    for (int k = 1; k < C::WK; ++k) {
+      x += *(const f4*)(q + k * (32 * PITCH));
+      y += *(const f4*)(q + k * (32 * PITCH) + 4);
+    }
+    *(f4*)&o[0] = x;
+    *(f4*)&o[4] = y;
+  };
 #pragma unroll
-    for (int q = 0; q < (TWO ? NI : 1); ++q) {
+  for (int q = 0; q < (TWO ? NI : 1); ++q) {
+    const int64_t n = n0 + (EPI == E_GATE ? wn * 32 : EPI == E_GATE2 ? wn * 64 + q * 32 : wn * 64) + nc;
+    const int nv = n >= N ? 0 : N - n < 8 ? (int)(N - n) : 8;
+    float b0[8] = {}, b1[8] = {};
+    if (EPI != E_DACT && !parts) {
+      if (P.bias0) load_n<T, 8>((const T*)P.bias0 + n, nv, b0);
+      if (PAIR && P.bias1) load_n<T, 8>((const T*)P.bias1 + n, nv, b1);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int64_t mi = m0 + wm * (MI * 32) + i * 32;
+      const T* extra = nullptr;                          // residual, or the mask
+      int64_t ldx = 0;
+      if constexpr (EPI == E_DACT) {
+        extra = (const T*)P.mask;
+        ldx = P.ldmask;
+      } else if (!parts) {
+        extra = (const T*)P.addend;
+        ldx = P.ldadd;
+      }
+      constexpr bool EARLY = !PAIR && (EPI != E_DACT || KIND != T_BIG);   // (the largest tile's products leave it no registers)
+      T pre[EARLY ? NP : 1][8];
+      if (EARLY && extra) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int64_t m = mi + row_of(p);
+          if (m < M && nv == 8) __builtin_memcpy(pre[p], extra + m * ldx + n, sizeof(pre[p]));
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -383,41 +430,22 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
       } else {
         __syncthreads();                                 // the sums of the waves that share the steps are added as they are read
       }
-      constexpr int LPR = PAIR ? 4 : 8;                  // lanes per row
+      // ---- first pass
+      const bool first = PAIR || (EPI == E_LIN && !parts && (act != DPVO_ACT_IDENTITY || P.save0)) || (EPI == E_DACT && !P.mask);
+      if (first) {
 #pragma unroll 1
-      for (int p = wk; p < 32 * LPR / 64; p += C::WK) {
-        const int rr = p * (64 / LPR) + lane / LPR, nc = lane % LPR * 8;
-        const int64_t m = m0 + wm * (MI * 32) + i * 32 + rr;
-        const int64_t n = n0 + (EPI == E_GATE ? wn * 32 : EPI == E_GATE2 ? wn * 64 + q * 32 : wn * 64) + nc;
-        if (m >= M || n >= N) continue;
-        const int nv = N - n < 8 ? (int)(N - n) : 8;
-        float v[8], u[8];
-        auto sums = [&](float (&o)[8], int at) BLK_INLINE {
-          const float* q = st - wk * (32 * PITCH) + rr * PITCH + at;
-          f4 x = *(const f4*)q, y = *(const f4*)(q + 4);
-#pragma unroll
-          for (int k = 1; k < C::WK; ++k) {
-            x += *(const f4*)(q + k * (32 * PITCH));
-            y += *(const f4*)(q + k * (32 * PITCH) + 4);
-          }
-          *(f4*)&o[0] = x;
-          *(f4*)&o[4] = y;
-        };
-        sums(v, nc);
-        if constexpr (PAIR) sums(u, 32 + nc);
-        if constexpr (EPI == E_DACT) {
-          if (P.mask) {
-            float h[8];
-            load_n<T, 8>((const T*)P.mask + m * P.ldmask + n, nv, h);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = h[e] > 0.f ? v[e] : 0.f;
-            store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
-          } else {
+        for (int p = 0; p < NP; ++p) {
+          const int rr = row_of(p);
+          const int64_t m = mi + rr;
+          if (m >= M || nv == 0) continue;
+          float v[8], u[8];
+          sums(v, rr, nc);
+          if constexpr (EPI == E_DACT) {
             float g[8], y[8];
             load_n<float, 8>(P.save0 + m * N + n, nv, g);
+            if (P.save1) load_n<float, 8>(P.save1 + m * N + n, nv, u);
             act_d_n<FINE, true, 8>(act, g, y);
             if (P.save1) {
-              load_n<float, 8>(P.save1 + m * N + n, nv, u);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 y[e] *= v[e];
@@ -428,34 +456,67 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= g[e];
             store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
-          }
-        } else if (EPI == E_LIN && P.part) {
-          store_n<float, 8>(P.part + ((int64_t)split * M + m) * N + n, nv, v);
-        } else {
-          float t[8];
-          if (P.bias0) {
-            load_n<T, 8>((const T*)P.bias0 + n, nv, t);
+          } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += t[e];
-          }
-          if (P.save0) store_n<float, 8>(P.save0 + m * N + n, nv, v);
-          act_n<FINE, true, 8>(act, v);
-          if constexpr (PAIR) {
-            if (P.bias1) {
-              load_n<T, 8>((const T*)P.bias1 + n, nv, t);
+            for (int e = 0; e < 8; ++e) v[e] += b0[e];
+            if (P.save0) store_n<float, 8>(P.save0 + m * N + n, nv, v);
+            act_n<FINE, true, 8>(act, v);
+            if constexpr (PAIR) {
+              sums(u, rr, 32 + nc);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) u[e] += t[e];
+              for (int e = 0; e < 8; ++e) u[e] += b1[e];
+              if (P.save1) store_n<float, 8>(P.save1 + m * N + n, nv, u);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] *= u[e];
             }
-            if (P.save1) store_n<float, 8>(P.save1 + m * N + n, nv, u);
+            if constexpr (PAIR) {
+              if (extra) {
+                load_n<T, 8>(extra + m * ldx + n, nv, u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= u[e];
+                for (int e = 0; e < 8; ++e) v[e] += u[e];
+              }
+              store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
+            } else {
+              *(f4*)(st0 + rr * PITCH + nc) = *(const f4*)&v[0];
+              *(f4*)(st0 + rr * PITCH + nc + 4) = *(const f4*)&v[4];
+            }
           }
-          if (P.addend) {
-            load_n<T, 8>((const T*)P.addend + m * P.ldadd + n, nv, t);
+        }
+      }
+      // ---- second pass of one sum (each lane reads back what it wrote itself)
+      if (!PAIR && (EPI != E_DACT || P.mask)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += t[e];
+        for (int p = 0; p < NP; ++p) {
+          const int rr = row_of(p);
+          const int64_t m = mi + rr;
+          if (m < M && nv) {
+            float v[8];
+            if (first) {
+              *(f4*)&v[0] = *(const f4*)(st0 + rr * PITCH + nc);
+              *(f4*)&v[4] = *(const f4*)(st0 + rr * PITCH + nc + 4);
+            } else {
+              sums(v, rr, nc);
+              if constexpr (EPI == E_LIN)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += b0[e];
+            }
+            if (parts) {
+              store_n<float, 8>(P.part + ((int64_t)split * M + m) * N + n, nv, v);
+            } else {
+              if (extra) {
+                float t[8];
+                if (EARLY && nv == 8) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) t[e] = (float)pre[EARLY ? p : 0][e];
+                } else {
+                  load_n<T, 8>(extra + m * ldx + n, nv, t);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = EPI == E_DACT ? (t[e] > 0.f ? v[e] : 0.f) : v[e] + t[e];
+              }
+              store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
+            }
           }
-          store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
         }
       }
       if constexpr (C::WK == 1) {
@@ -465,6 +526,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
         __syncthreads();
       }
     }
+  }
 }
 
 // ---- few rows (M <= 64): the weights are read once and nothing else counts, so a workgroup takes 16 columns of C and its W waves share the
