@@ -163,34 +163,37 @@ def _dact(dy, gate, up, act):
 
 
 def _dx(pairs, addend=None, gate=None, up=None, mask=None, act=0):
-    """sum of a . w over `pairs`; -> dx, and with `up` the second gradient"""
-    p = L.GatedLinearDx()
-    keep = []
-    for i, (a, w) in enumerate(pairs):
-        a, lda = _rows(a)
-        w, ldw = _rows(w)
-        keep += [a, w]
-        p.a[i], p.b[i], p.lda[i], p.ldb[i], p.K[i] = _p(a), _p(w), lda, ldw, a.shape[1]
-    M, N = keep[0].shape[0], keep[1].shape[1]
-    ref = keep[0]
-    dx = torch.empty(M, N, dtype=ref.dtype, device=ref.device)
+    """sum of a . w over `pairs` (one or two); -> dx, and with `up` the second gradient"""
+    a0, lda0 = _rows(pairs[0][0])
+    w0, ldw0 = _rows(pairs[0][1])
+    a1 = w1 = None
+    lda1 = ldw1 = K1 = ldadd = ldmask = 0
+    if len(pairs) == 2:
+        a1, lda1 = _rows(pairs[1][0])
+        w1, ldw1 = _rows(pairs[1][1])
+        K1 = a1.shape[1]
+    M, K0 = a0.shape
+    N = w0.shape[1]
+    dx = torch.empty(M, N, dtype=a0.dtype, device=a0.device)
     dx2 = torch.empty_like(dx) if up is not None else None
     if addend is not None:
-        addend, p.ldadd = _rows(addend)
+        addend, ldadd = _rows(addend)
     if mask is not None:
-        mask, p.ldmask = _rows(mask)
-    p.addend, p.mask, p.gate, p.up, p.dx, p.dx2 = _p(addend), _p(mask), _p(gate), _p(up), _p(dx), _p(dx2)
-    p.lddx, p.M, p.N, p.dtype, p.activation = N, M, N, _DTYPES[ref.dtype], act
+        mask, ldmask = _rows(mask)
+    p = L.GatedLinearDx((a0.data_ptr(), _p(a1)), (w0.data_ptr(), _p(w1)), _p(addend), _p(mask), _p(gate), _p(up), dx.data_ptr(), _p(dx2), (lda0, lda1),
+                        (ldw0, ldw1), (K0, K1), ldadd, ldmask, N, M, N, _DTYPES[a0.dtype], act)
     lib = L.lib()
     n = lib.dpvo_gated_linear_dx_workspace_bytes(ctypes.byref(p))
-    ws = _scratch(n, ref.device)
-    L.check(lib.dpvo_gated_linear_dx(ctypes.byref(p), _p(ws), n, _stream(ref)), "dpvo_gated_linear_dx")
+    ws = _scratch(n, a0.device)
+    rc = lib.dpvo_gated_linear_dx(ctypes.byref(p), _p(ws), n, _stream(a0))
+    if rc:
+        L.check(rc, "dpvo_gated_linear_dx")
     return dx, dx2
 
 
 def _dw(jobs):
     """jobs: (gradient of the sums [M,N], input [M,K], want dw, want db) -> [(dw, db), ...]"""
-    p = L.GatedLinearDw()
+    pa, pb, pdw, pdb, la, lb, ns, ks = [], [], [], [], [], [], [], []
     keep, out = [], []
     for a, b, want_w, want_b in jobs:
         if not (want_w or want_b):
@@ -198,19 +201,28 @@ def _dw(jobs):
             continue
         a, lda = _rows(a)
         b, ldb = _rows(b)
-        i = p.n
-        dw = torch.empty(a.shape[1], b.shape[1], dtype=a.dtype, device=a.device)      # (db is made beside it)
-        db = torch.empty(a.shape[1], dtype=a.dtype, device=a.device) if want_b else None
-        keep += [a, b, dw]
+        N, K = a.shape[1], b.shape[1]
+        dw = torch.empty(N, K, dtype=a.dtype, device=a.device)               # (db is made beside it)
+        db = torch.empty(N, dtype=a.dtype, device=a.device) if want_b else None
+        keep += (a, b, dw)
         out.append((dw if want_w else None, db))
-        p.a[i], p.b[i], p.dw[i], p.db[i], p.lda[i], p.ldb[i], p.N[i], p.K[i] = _p(a), _p(b), _p(dw), _p(db), lda, ldb, a.shape[1], b.shape[1]
-        p.n = i + 1
-    if p.n:
-        p.M, p.dtype = keep[0].shape[0], _DTYPES[keep[0].dtype]
+        pa.append(a.data_ptr())
+        pb.append(b.data_ptr())
+        pdw.append(dw.data_ptr())
+        pdb.append(_p(db))
+        la.append(lda)
+        lb.append(ldb)
+        ns.append(N)
+        ks.append(K)
+    if keep:
+        a = keep[0]
+        p = L.GatedLinearDw(*map(tuple, (pa, pb, pdw, pdb, la, lb, ns, ks)), a.shape[0], len(pa), _DTYPES[a.dtype])
         lib = L.lib()
         n = lib.dpvo_gated_linear_dw_workspace_bytes(ctypes.byref(p))
-        ws = _scratch(n, keep[0].device)
-        L.check(lib.dpvo_gated_linear_dw(ctypes.byref(p), _p(ws), n, _stream(keep[0])), "dpvo_gated_linear_dw")
+        ws = _scratch(n, a.device)
+        rc = lib.dpvo_gated_linear_dw(ctypes.byref(p), _p(ws), n, _stream(a))
+        if rc:
+            L.check(rc, "dpvo_gated_linear_dw")
     return out
 
 
