@@ -203,13 +203,14 @@ struct NormPlan {
 };
 NormPlan norm_plan(const dpvo_residual_norm_t& p) {
   NormPlan n;
-  n.sh = norm_shape(p.D);
   n.shared = p.f && p.gate && p.groups < p.M;
+  n.sh = norm_shape(p, true, norm_sums(p, n.shared));
   n.groups = n.shared ? p.groups : 1;
   n.rpg = n.groups ? p.M / n.groups : 0;
   // 4096 waves, four to a SIMD: enough loads in flight for the memory, few enough that their partial rows stay a few per cent of the traffic
-  const int L = NORM_SHAPES[n.sh].L;
-  const int64_t want = L > 64 ? 4096 / (L / 64) : 1024, rounds = cdiv64(n.rpg, norm_slots(n.sh));
+  const int L = n.sh == NORM_WIDE ? 0 : NORM_SHAPES[n.sh].L;
+  // (wide rows: rows of 2048 columns' sums, two to four workgroups a compute unit; 4096 x 8192 bf16 221 us in 64 parts, 130 in 128, 138 in 256)
+  const int64_t want = n.sh == NORM_WIDE ? 128 : L > 64 ? 4096 / (L / 64) : 1024, rounds = cdiv64(n.rpg, norm_slots(n.sh));
   if (n.groups >= want) {
     n.bpg = 1;
     n.gpb = cdiv64(n.groups, want);
@@ -406,7 +407,8 @@ extern "C" size_t dpvo_gated_linear_dw_workspace_bytes(const dpvo_gated_linear_d
 }
 extern "C" int dpvo_gated_linear_dw(const dpvo_gated_linear_dw_t* p, void* ws, size_t ws_bytes, void* stream) {
   if (!dw_ok(p)) return DPVO_E_INVALID;
-  if (dpvo_gated_linear_dw_workspace_bytes(p) > ws_bytes) return DPVO_E_WORKSPACE;
+  const size_t need = dpvo_gated_linear_dw_workspace_bytes(p);
+  if (need > ws_bytes || (need && !ws)) return DPVO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   const Plan c0 = dw_plan(p);
   const int64_t splits = c0.splits;
@@ -447,29 +449,32 @@ extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {
   NormArgs a = {};
   a.p = *p;
   a.rows_per_gate = p->gate ? (uint32_t)(p->M / p->groups) : 1;
-  const int sh = norm_shape(p->D);
-  const int64_t want = cdiv64(p->M, norm_slots(sh));
-  return norm_run(a, sh, false, want < 8192 ? want : 8192, (hipStream_t)stream);
+  const int sh = norm_shape(*p, false, 0);
+  // (ragged rows profit from several to a workgroup, whose loads then run ahead: 4096 x 2333 bf16 49 against 57 us, 8192 x 1001 24 against 32; of
+  //  whole pieces 8192 x 4096 takes 73 us with a workgroup to a row, 79 with 2048 workgroups)
+  const int64_t want = cdiv64(p->M, norm_slots(sh)), most = p->D % 8 ? 2048 : 8192;
+  return norm_run(a, sh, false, want < most ? want : most, (hipStream_t)stream);
 }
 
 extern "C" size_t dpvo_residual_norm_backward_workspace_bytes(const dpvo_residual_norm_t* p) {
   if (norm_check(p) || p->M == 0) return 0;
   const NormPlan n = norm_plan(*p);
   const int64_t rows = (n.shared && p->dgate ? n.groups * n.bpg : 0) + n.blocks * ((p->dw != nullptr) + (p->db != nullptr) + (p->dpw != nullptr) + (p->dpb != nullptr));
-  return (size_t)(rows * p->D * 4);
+  return (size_t)(rows * p->D * 4 + (n.sh == NORM_WIDE && rows ? p->M * NORM_STATS * 4 : 0));
 }
 extern "C" int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* ws, size_t ws_bytes, void* stream) {
   int rc = norm_check(p);
   if (rc) return rc;
   if (p->ldx < p->D || (p->f && p->ldf < p->D) || (p->gate && p->ldgate < p->D) || (p->ds && p->ldds < p->D) || (p->dh && p->lddh < p->D)) return DPVO_E_INVALID;
   if ((!p->f && (p->df || p->dgate || p->dpw || p->dpb)) || (p->dgate && !p->gate) || (p->post == DPVO_NORM_NONE && (p->dpw || p->dpb))) return DPVO_E_INVALID;
-  if (dpvo_residual_norm_backward_workspace_bytes(p) > ws_bytes) return DPVO_E_WORKSPACE;
+  const size_t need = dpvo_residual_norm_backward_workspace_bytes(p);
+  if (need > ws_bytes || (need && !ws)) return DPVO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   NormArgs a = {};
   a.p = *p;
   ColArgs c = {};
   float* w = (float*)ws;
-  const NormPlan n = p->M ? norm_plan(*p) : NormPlan{norm_shape(p->D), 0, 0, 1, 1, 0, false};
+  const NormPlan n = p->M ? norm_plan(*p) : NormPlan{0, 0, 0, 1, 1, 0, false};
   a.shared = n.shared;
   a.groups = n.groups; a.rpg = n.rpg; a.gpb = n.gpb; a.bpg = n.bpg;
   auto job = [&](void* out, int type, int64_t outs, int64_t parts) {
@@ -485,6 +490,7 @@ extern "C" int dpvo_residual_norm_backward(const dpvo_residual_norm_t* p, void* 
   a.part_pb = job(p->dpb, p->w_dtype, 1, n.blocks);
   if (n.shared) a.part_gate = job(p->dgate, p->f_dtype, n.groups, n.bpg);
   else if (!p->M && p->dgate) job(p->dgate, p->f_dtype, p->groups, 0);
+  if (n.sh == NORM_WIDE && c.n) a.stats = w;
   if (p->M) {
     rc = norm_run(a, n.sh, true, n.blocks, s);
     if (rc) return rc;

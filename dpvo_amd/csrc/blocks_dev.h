@@ -1,4 +1,4 @@
-// blocks_dev.h -- what the gated feed-forward / residual-norm kernels (blocks_gemm.h, blocks_norm.hip, blocks.hip) share: the three element
+// blocks_dev.h -- what the gated feed-forward / residual-norm kernels (blocks_gemm.h, blocks_norm.h, blocks.hip) share: the three element
 // types, loads and stores that end at a row's end, the activations and their derivatives.  Sums, statistics and activations are f32 throughout.
 #pragma once
 #include "common.h"

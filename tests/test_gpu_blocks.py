@@ -395,6 +395,20 @@ def residual_norm_case(g, tx, tb, lead, D, kind, post, gate, gate_act, scale, us
     ((9,), 384, "layer", "layer", (), "sigmoid", 1.0, "sh"),
     ((6,), 2560, "layer", "layer", (6,), "sigmoid", 0.5, "sh"),
     ((3,), 10000, "layer", "layer", (3,), "sigmoid", 1.0, "h"),
+    # widths that end inside a lane's piece, of every number of lanes
+    ((70,), 5, "layer", "layer", (70,), "sigmoid", 1.0, "sh"),
+    ((70,), 253, "layer", "rms", (1,), "silu", 1.0, "sh"),
+    ((37,), 1003, "layer", "layer", (37,), "sigmoid", 1.0, "sh"),
+    ((21,), 1999, "rms", "layer", (1,), "sigmoid", 1.0, "sh"),
+    ((11,), 3001, "layer", "layer", (11,), "sigmoid", 1.0, "sh"),
+    # rows over a whole workgroup: many groups, parts of a group, one of the two results alone, no gate, no norm
+    ((140, 2), 4099, "layer", "layer", (140, 1), "sigmoid", 0.5, "sh"),
+    ((3, 100), 4104, "rms", "rms", (3, 1), "identity", 1.0, "sh"),
+    ((300,), 4097, "layer", "layer", (), "sigmoid", 1.0, "s"),
+    ((150,), 5000, "layer", None, None, "identity", 1.0, "h"),
+    ((20,), 8193, None, "layer", (1,), "relu", 1.0, "sh"),
+    ((30,), 4200, "layer", "layer", (1,), "sigmoid", 1.0, "sh"),
+    ((5,), 12001, "rms", "layer", (5,), "silu", 1.0, "sh"),
 ])
 def test_residual_norm(dev, tx, tb, lead, D, kind, post, gate, gate_act, scale, use):
     g = torch.Generator().manual_seed(D + len(lead))
