@@ -9,7 +9,10 @@
     residual_norm(x, f, w, b, gate=...)        s = x + scale * act(gate) * post(f);  h = norm(s)          after a block and before the next
 
 Operands are float16, bfloat16 or float32 CUDA tensors of one type (`residual_norm`: the stream x may be float32 beside a 16-bit branch);
-products run on the matrix cores, sums, statistics and activations are float32.  Everything runs on the current stream of the tensors' device.
+products run on the matrix cores, sums, statistics and activations are float32.  What enters a second matrix product is rounded to the operands'
+type, as the matrix cores take it: the hidden product act(..) * (..), and in the backward pass the gradients of the sums (which the activations'
+derivatives read in float32, as saved).  So a 16-bit block's results are a step or two of its type's rounding away from the formula's, and its
+gradients need the loss scaled as those of any 16-bit operands.  Everything runs on the current stream of the tensors' device.
 Gradients of first order are provided; results and gradients do not vary from run to run.  Autocast is not consulted.  A backward pass that is
 captured into a graph follows PyTorch's rule: no eager graph of the same leaves may be alive."""
 import ctypes
@@ -235,10 +238,6 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _shape(g, like):
-    return None if g is None else g.reshape(like)
-
-
 # ------------------------------------------------------------------------------------------------------------------ linear
 class _Linear(torch.autograd.Function):
     @staticmethod
@@ -246,7 +245,7 @@ class _Linear(torch.autograd.Function):
         with _on(x):
             y, pre, _ = _forward(x, w, b, act, save=act != 0)
         ctx.save_for_backward(x, w, pre)
-        ctx.act, ctx.shape = act, x.shape
+        ctx.act = act
         return _like(y, x, w.shape[0])
 
     @staticmethod
@@ -257,9 +256,9 @@ class _Linear(torch.autograd.Function):
         with _on(x):
             dy = _rows(dy)[0]
             d = dy if ctx.act == 0 else _dact(dy, pre, None, ctx.act)[0]
-            dx = _dx([(d, w)])[0] if need[0] else None
+            dx = _dx([(d, w)])[0].view(x.shape) if need[0] else None
             (dw, db), = _dw([(d, x, need[1], need[2])])
-        return _shape(dx, ctx.shape), dw, db, None
+        return dx, dw, db, None
 
 
 def linear(x, weight, bias=None, activation="identity"):

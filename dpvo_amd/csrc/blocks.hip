@@ -74,7 +74,7 @@ int split_sum(const SumArgs& a, int dtype, hipStream_t s) {
   return DPVO_OK;
 }
 
-// dpvo_gated_linear_dact: one pass, 8 elements a thread
+// dpvo_gated_linear_dact: one pass, 8 elements a thread; 45312 x 384 in f16 45 us, 244 MB at 5.4 TB/s
 template <class T> __global__ void __launch_bounds__(256) dact_kernel(const T* dy, int64_t lddy, const float* gate, const float* up, T* dg, T* du, int64_t ldo,
                                                                        int act, int64_t M, int64_t N) {
   const int64_t n8 = (N + 7) / 8, total = M * n8;
@@ -163,16 +163,17 @@ struct Plan {
 };
 inline int tile_size(int kind) { return kind == T_BIG ? 256 : kind == T_SMALL || kind == T_TINY ? 64 : 128; }
 // `count(t)`: tiles of t x t; nb: blocks of the summed index; cut: whether parts are possible.
-//  - 256 x 256 reads LDS least per product and gives 1095 Tflop/s (bf16, 8192 x 8192 x 4096) where 128 x 128 gives 885, so a round of the latter (two
-//    workgroups on each of 256 compute units) takes 0.62 of a round of the former (one): whichever needs less.  But nothing hides the epilogue of
-//    one workgroup alone: with 16 blocks it still wins (79.7 against 89.3 us, 4096 x 4096 x 1024 twice), with 6 or 12 it loses (65.2 against
-//    56.6 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
-//  - 128 x 128 wants its two workgroups: at 432 tiles it wins over 64 x 64 (15.7 against 20.6 us), at 256 it loses (19.1 against 18.0).
+//  - 256 x 256 reads LDS least per product and gives 1127 Tflop/s (bf16, 8192 x 8192 x 4096: 488 us) where 128 x 128 gives 897 (613 us), so a round
+//    of the latter (two workgroups on each of 256 compute units) takes 0.62 of a round of the former (one): whichever needs less.  But nothing
+//    hides the epilogue of one workgroup alone: with 16 blocks it still wins (73.2 against 86.0 us, 4096 x 4096 x 1024 twice), with 6 it loses
+//    (55.8 against 49.5 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
+//  - 128 x 128 wants its two workgroups: at 432 tiles it wins over 64 x 64 (16.6 against 20.4 us, 9216 x 768 x 384), at 256 it loses (20.7 against
+//    18.7, 2048 x 2048 x 1024).
 //  - Parts: towards two workgroups a compute unit, each with 12 blocks at least (a part costs a tile's write and read in f32, and all of them a
 //    launch); dw 384 x 384 over 45312 rows: 45 us in 56 parts, 56 in 64, 59 in 16.  Where that does not fill them, small tiles in parts of 4
 //    blocks at least: over 9216 rows 23 us in 21 parts, 25 with large tiles in 16.  Below 16 blocks a second launch costs more than it
 //    saves: 333 x 2048 x 768 8.6 us whole, 14.0 in three.
-//  - 64 x 64 by four waves where there are few: 1237 x 385 x 882 in f32 24 us against 40 with two waves, at 864 tiles 13.3 against 11.6.
+//  - 64 x 64 by four waves where there are few: 1237 x 385 x 882 in f32 24.6 us against 40.5 with two waves, at 864 tiles 13.3 against 11.6.
 template <class F> Plan plan(F count, int64_t nb, int dtype, bool cut) {
   const int64_t t = count(128);
   if (dtype != DPVO_F32 && nb >= 16 && cdiv64(count(256), 256) * 100 < cdiv64(t, 512) * 62) return {T_BIG, 1};
