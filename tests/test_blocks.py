@@ -176,6 +176,17 @@ def test_entries_check_their_arguments():
         assert rn(True, **bad) == INVALID, bad
     assert rn(True, dh=one, lddh=32, dw=one) == WORKSPACE
     assert rn(True, M=0) == 0
+    # a size without a workspace behind it
+    big = 1 << 40
+    q = L.GatedLinear(**{**ok, "M": 100, "N": 64, "K": 64 * 64, "ldx": 64 * 64, "ldwg": 64 * 64, "ldy": 64})
+    assert lib.dpvo_gated_linear(ctypes.byref(q), null, big, null) == WORKSPACE
+    q, _ = dx(M=64, N=64, K=(0, 64 * 64), lda=(0, 64 * 64), ldb=(0, 64), lddx=64)
+    assert lib.dpvo_gated_linear_dx(ctypes.byref(q), null, big, null) == WORKSPACE
+    q = L.GatedLinearDw((one,), (one,), (one,), (), (32,), (64,), (32,), (64,), 45312, 1, 0)
+    assert lib.dpvo_gated_linear_dw_workspace_bytes(ctypes.byref(q)) > 0 and lib.dpvo_gated_linear_dw(ctypes.byref(q), null, big, null) == WORKSPACE
+    for D in (32, 5000):
+        q = L.ResidualNorm(x=one, dh=one, dw=one, ldx=D, lddh=D, D=D, M=5, x_dtype=1, f_dtype=1, h_dtype=1, w_dtype=1, norm=1)
+        assert lib.dpvo_residual_norm_backward_workspace_bytes(ctypes.byref(q)) > 0 and lib.dpvo_residual_norm_backward(ctypes.byref(q), null, big, null) == WORKSPACE
 
 
 def test_structs_match_the_header(tmp_path):

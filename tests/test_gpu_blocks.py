@@ -653,6 +653,31 @@ def test_the_run_of_them_on_two_streams(dev, t):
             assert all(torch.equal(x, y) for x, y in zip(w, q))
 
 
+def test_two_threads(dev):
+    """steps from two host threads at once, each on its own stream: nothing is shared between calls"""
+    import threading
+    leaves = [block_leaves(t, M=120, D=384, F=700) for t in (F16, F32)]
+    want = [block_step(d) for d in leaves]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got[i].append(block_step(leaves[i]))
+            s.synchronize()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    for i in range(2):
+        assert len(got[i]) == 10 and all(torch.equal(x, y) for step in got[i] for x, y in zip(step, want[i]))
+
+
 def test_captured_graphs(dev):
     """two graphs of forward passes (with and without sums in parts) and one of a whole step, replayed in turn with eager calls between: every replay
     equals the eager result on the inputs of the moment"""
@@ -667,15 +692,16 @@ def test_captured_graphs(dev):
         return block_step({k: v.detach().requires_grad_() for k, v in d.items()})
 
     wide = {"x": torch.randn(64, 4096, device=dev).half()}
+    wider = {"x": torch.randn(64, 5001, device=dev)}
 
     def wide_step(d):
         x = d["x"].detach().requires_grad_()
-        w, b = torch.ones(4096, device=dev).half().requires_grad_(), torch.ones(4096, device=dev).half().requires_grad_()
+        w, b = (torch.ones_like(x[0]).detach().requires_grad_() for _ in range(2))
         s, h = blocks.residual_norm(x, x * 0.5, w, b, gate=w, post_norm="layer", post_weight=w, post_bias=b)
         return [h, *torch.autograd.grad([s, h], [x, w, b], [torch.ones_like(s), torch.ones_like(h)])]
 
     jobs = []
-    for f, d in ((forward, leaves), (step, leaves), (forward, {**leaves, "x": leaves["x"][:50].clone()}), (wide_step, wide)):
+    for f, d in ((forward, leaves), (step, leaves), (forward, {**leaves, "x": leaves["x"][:50].clone()}), (wide_step, wide), (wide_step, wider)):
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
