@@ -749,9 +749,10 @@ template <class NX, class NB, int I> int norm_go(const NormArgs& a, bool back, i
     if constexpr (S.L < 1024) hipLaunchKernelGGL((norm_kernel<NX, NB, S.L, S.ragged>), dim3((unsigned)blocks), dim3(T), 0, s, a);
   } else {
     auto k = norm_back_kernel<NX, NB, S.L, S.ragged>;
-    const int bytes = norm_sums(a.p, a.shared) * T * 8 * 4;   // up to 80 KB, 128 with 1024 lanes
-    if (bytes > 64 * 1024) {
-      const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    constexpr int one = T * 8 * 4, most = (S.L < 1024 ? 5 : 4) * one;   // 80 or 128 KB
+    const int bytes = norm_sums(a.p, a.shared) * one;
+    if (bytes > 64 * 1024) {                             // (always the same value: another thread may be about to launch)
+      const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e != hipSuccess) return (int)e;
     }
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(T), bytes, s, a);
