@@ -33,7 +33,7 @@ constexpr int NORM_STATS = 6;
 // How a row of D elements is spread: 8 on each of L lanes, which keeps the backward's arrays of them in registers.  Four or more rows share
 // a workgroup where L <= 64 (no barriers there).  RAGGED: D is no multiple of 8.  Rows of more than 4096 elements go to the wide kernels, except
 // that the backward of 16-bit ones of up to 8192, in whole pieces and with up to four sums in LDS, still fits 1024 lanes (4096 x 8192: 153 us, wide
-// 254; f32 streams spill there: 884 us, wide 350; the forward takes 73 and 76 us, at 4096 x 5120 82 and 50).
+// 254; f32 streams spill there: 884 us, wide 350; the forward takes 73 and 76 us, at 4096 x 5120 82 and 74).
 struct NormShape { int L; bool ragged; };
 constexpr NormShape NORM_SHAPES[] = {{16, false}, {32, false}, {64, false}, {128, false}, {256, false}, {512, false},
                                      {16, true}, {32, true}, {64, true}, {128, true}, {256, true}, {512, true}, {1024, false}};
@@ -733,7 +733,8 @@ template <class NX, class NB> __global__ void __launch_bounds__(256, 2) norm_col
 }
 
 // (512 threads with 16 elements each where those are enough: two workgroups on a compute unit take turns at their barriers.  4096 x 8192 bf16, forward and
-// first backward kernel: 87 and 145 us, 101 and 215 with 1024 threads of 8; 2048 x 16384: 92 and 170 with 1024 of 16, 121 and 199 with 512 of 32)
+// first backward kernel: 87 and 145 us, 101 and 215 with 1024 threads of 8; 2048 x 16384: 92 and 170 with 1024 of 16, 121 and 199 with 512 of 32.
+// Since whole pieces have kernels of their own: 75 and 126, 73 and 143)
 template <class NX, class NB, int L, bool RAGGED> int norm_wide(const NormArgs& a, bool back, int64_t blocks, hipStream_t s) {
   const dim3 rows((unsigned)(a.p.M < 8192 ? a.p.M : 8192));
   if (!back) hipLaunchKernelGGL((norm_wide_kernel<NX, NB, L, 2, RAGGED>), rows, dim3(L), 0, s, a);
