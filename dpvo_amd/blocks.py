@@ -146,7 +146,7 @@ def _forward(x, wg, bg, act, v=None, wu=None, bu=None, residual=None, save=False
     p = L.GatedLinear(_p(x), _p(v) if wu is not None else None, _p(wg), _p(wu), _p(bg), _p(bu), _p(residual), _p(y), _p(sg), _p(su), ldx, ldv,
                       ldwg, ldwu, ldr, N, M, N, x.shape[1], Kv, _DTYPES[x.dtype], act)
     lib, n, ws = L.lib(), 0, None
-    if act == 0 and wu is None and M > 64:                       # (few rows: never in parts)
+    if act == 0 and wu is None and M > 16:                       # (few rows: never in parts)
         n = lib.dpvo_gated_linear_workspace_bytes(ctypes.byref(p))
         ws = _scratch(n, x.device)
     rc = lib.dpvo_gated_linear(ctypes.byref(p), _p(ws), n, _stream(x))

@@ -246,14 +246,29 @@ int norm_run(const NormArgs& a, int sh, bool back, int64_t blocks, hipStream_t s
 
 using namespace blk;
 
-// A plain projection (no activation, nothing saved) of more rows than the few-row kernel takes may be cut into parts like a gradient's sum
+// A plain projection (no activation, nothing saved) may be cut into parts like a gradient's sum
+static bool linear_cut(const dpvo_gated_linear_t* p) {
+  return !p->w_up && p->activation == DPVO_ACT_IDENTITY && !p->save_gate && p->ldy == p->N && (!p->residual || p->ldr == p->N);
+}
 static Plan linear_plan(const dpvo_gated_linear_t* p, int epi) {
   const int bk = block_k(p->dtype);
-  const bool cut = epi == E_LIN && p->activation == DPVO_ACT_IDENTITY && !p->save_gate && p->ldy == p->N && (!p->residual || p->ldr == p->N);
   Plan c = plan([&](int t) { return tiles(p->M, epi == E_GATE ? 2 * p->N : p->N, t); }, cdiv64(p->K, bk) + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0),
-                p->dtype, cut);
+                p->dtype, linear_cut(p));
   if (epi == E_GATE2 && c.kind == T_BIG) c.kind = T_TILE;      // (two sets of sums do not fit the registers of the largest tile)
   return c;
+}
+// The few-row kernel's workgroups (64 rows x 16 columns) instead of tiles: up to 16 rows, and wherever they are one to a compute unit at most (f16
+// 200 x 1024 x 1024 relu 7.5 against 10.3 us, with 384 of them 12.7 against 10.5); twice as many up to 32 rows, where half of their products are
+// for nothing but the weights' bytes count, and for two inputs in f32 (200 x 384 x 384 10.7 against 24.2 us, with 384 of them 18.6 against
+// 24.3, with 768 28.1 against 25.0).  Beyond 16 rows not
+//  - for 16-bit rows of odd length, whose unaligned pieces the tiles load once and these workgroups again and again (96 x 882 x 385: 14.9 against
+//    9.0 us, with 386 columns 7.7 against 8.1; by the length and not the address, so that a result does not depend on where its operands lie),
+//  - for long sums that may be cut into parts (f16 96 x 1024 x 4096: 20.1 against 14.8 us, 96 x 768 x 2048 11.5 against 11.8).
+static bool linear_few(const dpvo_gated_linear_t* p, int epi) {
+  if (p->M <= 16) return true;
+  if (cdiv64(p->N, 16) * cdiv64(p->M, 64) > (p->M <= 32 || (epi == E_GATE2 && p->dtype == DPVO_F32) ? 512 : 256)) return false;
+  if (p->dtype != DPVO_F32 && (p->K % 2 || (p->w_up && p->Kv % 2))) return false;
+  return !(linear_cut(p) && p->K > 2048);
 }
 static int linear_epi(const dpvo_gated_linear_t* p) {
   if (!p->w_up) return E_LIN;
@@ -261,7 +276,8 @@ static int linear_epi(const dpvo_gated_linear_t* p) {
 }
 
 extern "C" size_t dpvo_gated_linear_workspace_bytes(const dpvo_gated_linear_t* p) {
-  if (!p || !type_ok(p->dtype) || p->M <= FEW_ROWS || p->N <= 0 || p->K < 0 || p->Kv < 0 || p->w_up) return 0;
+  if (!p || !type_ok(p->dtype) || p->M <= 0 || p->N <= 0 || p->K < 0 || p->Kv < 0 || p->w_up) return 0;
+  if (linear_few(p, E_LIN)) return 0;
   const Plan c = linear_plan(p, E_LIN);
   return c.splits > 1 ? (size_t)(c.splits * p->M * p->N * 4) : 0;
 }
@@ -286,7 +302,7 @@ extern "C" int dpvo_gated_linear(const dpvo_gated_linear_t* p, void* ws, size_t 
   q.act = p->activation; q.splits = 1;
   q.nb0 = cdiv64(p->K, bk);
   q.nb = q.nb0 + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0);
-  if (p->M <= FEW_ROWS) return gemm(a, p->dtype, F_NT, epi, T_FEW, cdiv64(p->N, 16), s);
+  if (linear_few(p, epi)) return gemm(a, p->dtype, F_NT, epi, T_FEW, cdiv64(p->N, 16), s);
   const Plan c = linear_plan(p, epi);
   const int64_t n = tiles_of(q, c.kind, epi == E_GATE ? 2 : 1);
   if (c.splits == 1) return gemm(a, p->dtype, F_NT, epi, c.kind, n, s);

@@ -148,7 +148,6 @@ struct GemmArgs {
 
 // how a product is run: tiles of 128 x 128, 256 x 256 or 64 x 64 (by two waves or four), or few rows with the summed index over the waves (blocks_gemm.h)
 enum { T_TILE = 0, T_BIG = 1, T_SMALL = 2, T_TINY = 3, T_FEW = 4 };
-constexpr int FEW_ROWS = 64;
 
 int gemm_f16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);
 int gemm_bf16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);

@@ -536,7 +536,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
   }
 }
 
-// ---- few rows (M <= 64): the weights are read once and nothing else counts, so a workgroup takes 16 columns of C and its W waves share the
+// ---- few rows: the weights are read once (for 64 rows) and little else counts, so a workgroup takes 16 columns of C and its W waves share the
 // summed index; each lane loads its 16 bytes of a weight row straight into the matrix instruction's operand (16x16, the weight's 16 rows on
 // the first side), a batch of loads at a time.  The waves' sums meet in LDS and are added in the waves' order.
 // One row of bf16, 2 x 4096 x 1024 and 1024 x 4096: 5.6 us (17 MB at 3.0 TB/s) and 7.8 us (8 MB: 64 workgroups only, each a chain of 8 KB of loads per wave).
@@ -608,7 +608,7 @@ template <int EPI, int MT, int W> __global__ void __launch_bounds__(64 * W) __at
   __shared__ f4 red[W][NA][MT][64];
   const Prob& P = args.p[0];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
-  const int64_t M = P.M, N = P.N, n0 = (int64_t)blockIdx.x * 16;
+  const int64_t M = P.M, N = P.N, n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
   const int64_t wr = n0 + lr < N ? n0 + lr : N - 1;      // columns behind N, rows behind M: the last again, not stored
   f4 acc[NA][MT];
 #pragma unroll
@@ -618,7 +618,7 @@ template <int EPI, int MT, int W> __global__ void __launch_bounds__(64 * W) __at
   auto rows = [&](const T* (&x)[MT], int seg) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int64_t m = i * 16 + lr < M ? i * 16 + lr : M - 1;
+      const int64_t m = m0 + i * 16 + lr < M ? m0 + i * 16 + lr : M - 1;
       x[i] = (const T*)P.A[seg] + m * P.lda[seg] + lq * KE;
     }
   };
@@ -648,7 +648,7 @@ template <int EPI, int MT, int W> __global__ void __launch_bounds__(64 * W) __at
   __syncthreads();
   for (int q = threadIdx.x; q < MT * 64; q += 64 * W) {
     const int i = q >> 6, l = q & 63;
-    const int64_t m = i * 16 + (l & 15), n = n0 + (l >> 4) * 4;
+    const int64_t m = m0 + i * 16 + (l & 15), n = n0 + (l >> 4) * 4;
     if (m >= M || n >= N) continue;
     const int nv = N - n < 4 ? (int)(N - n) : 4;
     float v[NA][4], t[4];
@@ -682,7 +682,7 @@ template <int EPI> int few(const GemmArgs& a, int64_t blocks, hipStream_t s) {
   const Prob& p = a.p[0];
   const int64_t K = p.K[0] > p.K[1] ? p.K[0] : p.K[1];
   // 16 waves where 4 would each have more than one batch of eight steps to wait for
-  if (p.M > 16) hipLaunchKernelGGL((few_kernel<EPI, 4, 8>), dim3((unsigned)blocks), dim3(512), 0, s, a);
+  if (p.M > 16) hipLaunchKernelGGL((few_kernel<EPI, 4, 8>), dim3((unsigned)blocks, (unsigned)cdiv64(p.M, 64)), dim3(512), 0, s, a);
   else if (K > 4 * 8 * 4 * KE) hipLaunchKernelGGL((few_kernel<EPI, 1, 16>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
   else hipLaunchKernelGGL((few_kernel<EPI, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a);
   DPVO_LAUNCH_CHECK();

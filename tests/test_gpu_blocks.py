@@ -114,7 +114,7 @@ def layer(g, n, k, t, bias=True, grad=True):
 TYPES = [F16, BF16, F32]
 # (M, K, N): single elements, single tokens, below / at / above a tile and a block of the sum, odd everything
 SIZES = [(1, 1, 1), (1, 384, 384), (2, 7, 5), (3, 65, 130), (16, 64, 128), (33, 33, 31), (96, 384, 385), (128, 128, 128), (129, 63, 257),
-         (300, 882, 100), (640, 200, 72)]
+         (300, 882, 100), (640, 200, 72), (70, 385, 882), (100, 2500, 64), (1300, 90, 330), (1100, 600, 300), (2900, 100, 900)]
 
 
 # ------------------------------------------------------------------------------------------------------------------ linear
