@@ -13,11 +13,12 @@ products run on the matrix cores, sums, statistics and activations are float32. 
 type, as the matrix cores take it: the hidden product act(..) * (..), and in the backward pass the gradients of the sums (which the activations'
 derivatives read in float32, as saved).  So a 16-bit block's results are a step or two of its type's rounding away from the formula's, and its
 gradients need the loss scaled as those of any 16-bit operands.  Everything runs on the current stream of the tensors' device.
-Gradients of first order are provided; results and gradients do not vary from run to run.  Autocast is not consulted.  A backward pass that is
+Gradients of first order are provided, in reverse mode (dual tensors are refused); results and gradients do not vary from run to run.  Autocast is not consulted.  A backward pass that is
 captured into a graph follows PyTorch's rule: no eager graph of the same leaves may be alive."""
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -42,8 +43,17 @@ def _code(table, key, what, arg):
         _fail(what, f"{arg} is {key!r}, not one of {', '.join(map(repr, table))}")
 
 
+def _check_plain(what, *tensors):
+    """the kernels read and write memory behind torch's back: refuses what would get lost there"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail(what, "forward-mode derivatives are not provided, and an input is a dual tensor")
+
+
 def _check(what, x, *others):
     """one device, a dtype that the kernels know"""
+    _check_plain(what, x, *others)
     for t in others:
         if t is not None and t.device != x.device:
             _fail(what, f"tensors on {x.device} and {t.device}")
@@ -251,6 +261,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_plain("linear", dy)
         x, w, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         with _on(x):
@@ -288,6 +299,7 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_plain("gated_linear", dy)
         x, v, wg, wu, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dv = dwg = dwu = dbg = dbu = None
@@ -342,6 +354,7 @@ class _FeedForward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_plain("gated_feed_forward", dy)
         x, wg, wu, wd, h, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dwu = dbg = dbu = None
@@ -396,6 +409,7 @@ class _GatedResidual(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_plain("gated_residual", dy)
         x, wg, w1, w2, t, g, r = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dbg = dw1 = db1 = dw2 = db2 = None
@@ -494,6 +508,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, ds, dh):
+        _check_plain("residual_norm", ds, dh)
         x, f, gate, w, b, pw, pb = ctx.saved_tensors
         grads = [None] * 7
         if ds is None and dh is None:

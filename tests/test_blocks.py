@@ -218,3 +218,47 @@ def test_state_dict_keys_stay():
     keys = list(N.Update(3).gru.state_dict())
     assert keys == ["0.weight", "0.bias"] + [f"1.{k}.{w}" for k in ("gate.0", "res.0", "res.2") for w in ("weight", "bias")] + ["2.weight", "2.bias"] + \
         [f"3.{k}.{w}" for k in ("gate.0", "res.0", "res.2") for w in ("weight", "bias")]
+
+
+# ------------------------------------------------------------------------------------------------------------------ what torch records elsewhere
+# every operator with tensors t(name, shape) in the place of its inputs: `make(f)` is one call with f around the named one
+CALLS = [
+    ("linear", lambda t: blocks.linear(t("x", 3, 4), t("w", 5, 4), t("b", 5))),
+    ("gated_linear", lambda t: blocks.gated_linear(t("x", 3, 4), t("w", 5, 4), t("wu", 5, 4), t("b", 5), t("bu", 5), up_input=t("v", 3, 4), residual=t("r", 3, 5))),
+    ("gated_feed_forward", lambda t: blocks.gated_feed_forward(t("x", 3, 4), t("w", 5, 4), t("wu", 5, 4), t("wd", 4, 5), t("b", 5), t("bu", 5), t("bd", 4))),
+    ("gated_residual", lambda t: blocks.gated_residual(t("x", 3, 4), t("w", 4, 4), t("b", 4), t("w1", 6, 4), t("b1", 6), t("w2", 4, 6), t("b2", 4))),
+    ("norm", lambda t: blocks.norm(t("x", 3, 4), t("w", 4), t("b", 4))),
+    ("residual_norm", lambda t: blocks.residual_norm(t("x", 3, 4), t("f", 3, 4), t("w", 4), t("b", 4), gate=t("gate", 4), post_norm="layer",
+                                                     post_weight=t("pw", 4), post_bias=t("pb", 4))),
+]
+
+
+def names_of(call):
+    names = []
+
+    def t(name, *shape):
+        names.append(name)
+        return z(*shape)
+    with pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+        call(t)
+    return names
+
+
+@pytest.mark.parametrize("what,call", CALLS, ids=[c[0] for c in CALLS])
+def test_forward_mode_is_refused(what, call):
+    """a dual tensor in any place: its tangent would be dropped"""
+    from torch.autograd import forward_ad as fw
+    for grad in (False, True):
+        for name in names_of(call):
+            with fw.dual_level(), pytest.raises(L.DPVOHipError, match="forward-mode"):
+                call(lambda n, *s: fw.make_dual(z(*s, requires_grad=grad), torch.ones(*s)) if n == name else z(*s))
+    with fw.dual_level(), pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+        call(lambda n, *s: z(*s))                                               # a level alone is no dual tensor
+
+
+@pytest.mark.parametrize("f,n", [(blocks._Linear, 1), (blocks._GatedLinear, 1), (blocks._FeedForward, 1), (blocks._GatedResidual, 1), (blocks._ResidualNorm, 2)])
+def test_forward_mode_of_a_backward_is_refused(f, n):
+    """... and as the gradient that arrives"""
+    from torch.autograd import forward_ad as fw
+    with fw.dual_level(), torch.no_grad(), pytest.raises(L.DPVOHipError, match="forward-mode"):
+        f.backward.__wrapped__(None, *[fw.make_dual(z(3, 4), torch.ones(3, 4)) for _ in range(n)])
