@@ -43,12 +43,17 @@ def _code(table, key, what, arg):
         _fail(what, f"{arg} is {key!r}, not one of {', '.join(map(repr, table))}")
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
 def _check_plain(what, *tensors):
     """the kernels read and write memory behind torch's back: refuses what would get lost there"""
     if forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 _fail(what, "forward-mode derivatives are not provided, and an input is a dual tensor")
+    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
+        _fail(what, "a call under torch.jit.trace or make_fx: what the kernels write is not recorded, a trace would return memory as it was")
 
 
 def _check(what, x, *others):

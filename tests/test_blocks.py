@@ -262,3 +262,16 @@ def test_forward_mode_of_a_backward_is_refused(f, n):
     from torch.autograd import forward_ad as fw
     with fw.dual_level(), torch.no_grad(), pytest.raises(L.DPVOHipError, match="forward-mode"):
         f.backward.__wrapped__(None, *[fw.make_dual(z(3, 4), torch.ones(3, 4)) for _ in range(n)])
+
+
+@pytest.mark.parametrize("what,call", CALLS, ids=[c[0] for c in CALLS])
+def test_traces_are_refused(what, call):
+    """torch.jit.trace and make_fx would record the outputs' allocation and nothing that fills it"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f = lambda x: call(lambda n, *s: x if n == "x" else z(*s))  # noqa: E731
+    with torch.no_grad():
+        with pytest.raises(L.DPVOHipError, match="jit.trace"):
+            torch.jit.trace(f, z(3, 4))
+        for mode in ("real", "fake", "symbolic"):
+            with pytest.raises(L.DPVOHipError, match="make_fx"):
+                make_fx(f, tracing_mode=mode)(z(3, 4))
