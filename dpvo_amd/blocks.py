@@ -54,6 +54,9 @@ def _check_plain(what, *tensors):
                 _fail(what, "forward-mode derivatives are not provided, and an input is a dual tensor")
     if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
         _fail(what, "a call under torch.jit.trace or make_fx: what the kernels write is not recorded, a trace would return memory as it was")
+    for t in tensors:
+        if type(t) is not torch.Tensor and t is not None and type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+            _fail(what, f"a {type(t).__name__}, whose values do not lie in memory of its own")
 
 
 def _check(what, x, *others):

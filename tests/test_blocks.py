@@ -275,3 +275,33 @@ def test_traces_are_refused(what, call):
         for mode in ("real", "fake", "symbolic"):
             with pytest.raises(L.DPVOHipError, match="make_fx"):
                 make_fx(f, tracing_mode=mode)(z(3, 4))
+
+
+class Elsewhere(torch.Tensor):
+    """a tensor without memory: its values are another tensor's"""
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(func)
+
+
+@pytest.mark.parametrize("what,call", CALLS, ids=[c[0] for c in CALLS])
+def test_tensors_without_memory_are_refused(what, call):
+    """an address of 0 would stand for a parameter that is not there"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    for name in names_of(call):
+        with pytest.raises(L.DPVOHipError, match="a Elsewhere, whose values"):
+            call(lambda n, *s: Elsewhere(z(*s)) if n == name else z(*s))
+    with FakeTensorMode(), pytest.raises(L.DPVOHipError, match="FakeTensor"):
+        call(lambda n, *s: z(*s))
+
+    class Named(torch.Tensor):                                                  # a subclass in name only is an ordinary tensor
+        pass
+    with pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+        call(lambda n, *s: z(*s).as_subclass(Named) if n in "xw" else torch.nn.Parameter(z(*s)))
