@@ -88,7 +88,10 @@ def _features(what, x):
 
 # ------------------------------------------------------------------------------------------------------------------ launches
 def _rows(t):
-    """[..., K] as rows whose elements are contiguous: (tensor [M,K], leading dimension); a copy only where no such view exists"""
+    """[..., K] as rows whose elements are contiguous: (tensor [M,K], leading dimension); a copy only where no such view exists, or where the sign
+    is pending (the gradient that comes back through a complex conjugate's imaginary part is a negated view; one of a single feature has rows)"""
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         K = t.shape[-1]
         return t if t.dim() == 2 else t.view(-1 if K else t.numel(), K), K
@@ -108,7 +111,11 @@ def _rows(t):
 
 
 def _vector(t):
-    return t if t is None or t.stride(0) == 1 or t.shape[0] <= 1 else t.contiguous()
+    if t is None:
+        return t
+    if t.is_neg():
+        t = t.resolve_neg()
+    return t if t.stride(0) == 1 or t.shape[0] <= 1 else t.contiguous()
 
 
 def _p(t):

@@ -305,3 +305,17 @@ def test_tensors_without_memory_are_refused(what, call):
         pass
     with pytest.raises(L.DPVOHipError, match="run on the GPU only"):
         call(lambda n, *s: z(*s).as_subclass(Named) if n in "xw" else torch.nn.Parameter(z(*s)))
+
+
+def test_pending_signs_are_resolved():
+    """a negated view: its memory holds the values with the other sign"""
+    for shape in ((4, 6), (2, 3, 6), (1, 6), (6,), (4, 1), (2, 3, 1), (1,)):
+        x = torch.randn(*shape)
+        for neg in (torch._neg_view(x), torch.complex(x, x).conj().imag):
+            assert neg.is_neg()
+            for t in (neg, neg[..., ::2], neg[..., :5]):
+                r, ld = blocks._rows(t)
+                assert not r.is_neg() and ld >= r.shape[1] and torch.equal(r, t.reshape(-1, t.shape[-1]))
+                if t.dim() == 1:
+                    r = blocks._vector(t)
+                    assert not r.is_neg() and torch.equal(r, t)

@@ -841,3 +841,31 @@ def test_gru_is_the_stage_of_the_tracker(dev):
             N.linear(fg[:, :384], W2, b2, out=z, epilogue=N.EPI_GATED, gate=fg[:, 384:])
     # roundings per block: operand h, weights, the hidden layer, the gate, twice over; each half a step (2^-11) of values of a few units
     assert float((y[0] - z).abs().max()) < 16 * 2.0 ** -11 * float(z.abs().max())
+
+
+@pytest.mark.parametrize("D", [1, 20])
+def test_pending_signs(dev, D):
+    """inputs that are negated views, and the gradient that a complex conjugate sends back: a negated view too, with rows where D is 1"""
+    g = torch.Generator().manual_seed(11)
+    neg = lambda t: torch._neg_view(-t)  # noqa: E731
+    x, n, e, f, r = make(g, 9, D, grad=False), make(g, D, grad=False), make(g, D, grad=False), make(g, 9, D, grad=False), make(g, 9, 12, grad=False)
+    w, wu, b, wd, sq = (make(g, *s, grad=False) for s in ((12, D), (12, D), (12,), (D, 12), (D, D)))
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    runs = [(lambda x, sq, e: blocks.linear(x, sq, e, "silu"), (x, sq, e)),
+            (lambda x, w, c, b, r: blocks.gated_linear(x, w, c, b, b, residual=r), (x, w, wu, b, r)),
+            (lambda x, w, c, d, b, e: blocks.gated_feed_forward(x, w, c, d, b, b, e), (x, w, wu, wd, b, e)),
+            (lambda x, sq, e, w, b, d: blocks.gated_residual(x, sq, e, w, b, d, e), (x, sq, e, w, b, wd)),
+            (lambda x, n, e: blocks.norm(x, n, e, "rms"), (x, n, e)),
+            (lambda x, f, n, e: blocks.residual_norm(x, f, n, e, gate=n, post_norm="rms", post_weight=e)[1], (x, f, n, e))]
+    for k, (run, args) in enumerate(runs):
+        want = [t.clone().requires_grad_() for t in args]
+        got = [neg(t).requires_grad_() for t in args]
+        y0, y1 = run(*want), run(*got)
+        assert torch.equal(y0, y1), k
+        dy = torch.randn(y0.shape, generator=g).cuda()
+        for p, q in zip(torch.autograd.grad(y0, want, dy), torch.autograd.grad(y1, got, neg(dy))):
+            assert torch.equal(p, q), k
+        # the imaginary part of a conjugate is minus the values
+        p, = torch.autograd.grad((run(*want) * dy).sum(), want[:1])
+        q, = torch.autograd.grad((torch.complex(dy, run(*want)).conj().imag * -dy).sum(), want[:1])
+        assert torch.equal(p, q), k
