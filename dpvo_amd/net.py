@@ -129,6 +129,27 @@ class GradientClip(nn.Module):
         return x
 
 
+def _read(m, cls):
+    """a child whose parameters are read in place of a call: refused if a call would do anything else (another forward, hooks)"""
+    d = m.__dict__
+    if (type(m) is not cls and (not isinstance(m, cls) or type(m).forward is not cls.forward)) or d["_forward_hooks"] or d["_forward_pre_hooks"] or \
+            d["_backward_hooks"] or d["_backward_pre_hooks"] or "forward" in d:
+        raise L.DPVOHipError(f"the block's own kernels take the place of this child's call, which must be that of a {cls.__name__} without hooks: {m}")
+    return m
+
+
+def _read_all(seq, classes):
+    m = list(_read(seq, nn.Sequential)._modules.values())
+    if len(m) != len(classes):
+        raise L.DPVOHipError(f"the block's own kernels take the place of {', '.join(c.__name__ for c in classes)}, not of {seq}")
+    for c, cls in zip(m, classes):
+        _read(c, cls)
+    return m
+
+
+_GATE, _RES = (nn.Linear, nn.Sigmoid), (nn.Linear, nn.ReLU, nn.Linear)
+
+
 class GatedResidual(nn.Module):
     def __init__(self, dim):
         super().__init__()
@@ -136,9 +157,11 @@ class GatedResidual(nn.Module):
         self.res = nn.Sequential(nn.Linear(dim, dim), nn.ReLU(inplace=True), nn.Linear(dim, dim))
 
     def forward(self, x):
-        """x + gate(x) * res(x) (dpvo/blocks.py:23-24), differentiable; runs in x's dtype (f32 as the reference trains, or f16 / bf16)"""
-        gate, first, last = self.gate[0], self.res[0], self.res[2]
-        to = lambda t: t.to(x.dtype)
+        """x + gate(x) * res(x) (dpvo/blocks.py:23-24), differentiable; runs in x's dtype (f32 as the reference trains, or f16 / bf16).
+        The children's parameters are read (parametrized ones too), their calls do not happen: one with hooks or another forward is refused"""
+        gate, _ = _read_all(self.gate, _GATE)
+        first, _, last = _read_all(self.res, _RES)
+        to = lambda t: None if t is None else t.to(x.dtype)
         return blocks.gated_residual(x, to(gate.weight), to(gate.bias), to(first.weight), to(first.bias), to(last.weight), to(last.bias))
 
 
@@ -148,7 +171,12 @@ class GatedStack(nn.Sequential):
 
     def forward(self, x):
         for m in self:
-            x = blocks.norm(x, m.weight, m.bias, "layer", m.eps) if isinstance(m, nn.LayerNorm) else m(x)
+            if isinstance(m, nn.LayerNorm):
+                if _read(m, nn.LayerNorm).normalized_shape != x.shape[-1:]:
+                    raise L.DPVOHipError(f"{m} for rows of {tuple(x.shape[-1:])}")
+                x = blocks.norm(x, m.weight, m.bias, "layer", m.eps)
+            else:
+                x = m(x)
         return x
 
 

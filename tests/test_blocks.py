@@ -319,3 +319,68 @@ def test_pending_signs_are_resolved():
                 if t.dim() == 1:
                     r = blocks._vector(t)
                     assert not r.is_neg() and torch.equal(r, t)
+
+
+# ------------------------------------------------------------------------------------------------------------------ the model's modules
+def plain_blocks(monkeypatch):
+    """the two operators that the model's stage calls, in torch on the host: what surrounds them is tested here"""
+    F = torch.nn.functional
+    monkeypatch.setattr(blocks, "norm", lambda x, w, b, kind, eps: F.layer_norm(x, x.shape[-1:], w, b, eps))
+    monkeypatch.setattr(blocks, "gated_residual", lambda x, wg, bg, w1, b1, w2, b2: x + torch.sigmoid(F.linear(x, wg, bg)) * F.linear(F.relu(F.linear(x, w1, b1)), w2, b2))
+
+
+class Adapter(torch.nn.Linear):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+def hooked(register):
+    def change(gru):
+        getattr(gru[1].res[2], register)(lambda *a: None)
+    return change
+
+
+def replaced(path, module):
+    def change(gru):
+        *up, last = path.split(".")
+        setattr(gru.get_submodule(".".join(up)) if up else gru, last, module)
+    return change
+
+
+@pytest.mark.parametrize("change", [
+    hooked("register_forward_hook"), hooked("register_forward_pre_hook"), hooked("register_full_backward_hook"), hooked("register_full_backward_pre_hook"),
+    lambda gru: gru[3].gate.register_forward_hook(lambda *a: None), lambda gru: gru[1].gate[1].register_forward_hook(lambda *a: None),
+    lambda gru: gru[2].register_forward_hook(lambda *a: None), lambda gru: torch.nn.utils.weight_norm(gru[1].res[0]),
+    replaced("1.gate.0", Adapter(384, 384)), replaced("1.res.2", torch.nn.Identity()), replaced("1.gate.1", torch.nn.Tanh()), replaced("3.res.1", torch.nn.GELU()),
+    replaced("1.res", torch.nn.Sequential(torch.nn.Linear(384, 384), torch.nn.ReLU(), torch.nn.Dropout(), torch.nn.Linear(384, 384))),
+    replaced("0", type("Norm", (torch.nn.LayerNorm,), {"forward": lambda self, x: x})(384)), replaced("0", torch.nn.LayerNorm((2, 384), elementwise_affine=False)),
+    lambda gru: setattr(gru[1].res[0], "forward", lambda x: x),
+])
+def test_children_that_would_do_something_else_are_refused(change, monkeypatch):
+    """the stage reads its children's parameters and does not call them"""
+    from dpvo_amd import net as N
+    plain_blocks(monkeypatch)
+    gru = N.Update(3).gru
+    gru(z(2, 384))
+    change(gru)
+    with pytest.raises(L.DPVOHipError):
+        gru(z(2, 384))
+
+
+def test_children_that_are_read(monkeypatch):
+    """no bias, a parametrized weight, a subclass with the same forward, hooks on the block itself: what a call of them would give"""
+    from dpvo_amd import net as N
+    plain_blocks(monkeypatch)
+    torch.manual_seed(0)
+    gru, x, seen = N.Update(3).gru, torch.randn(5, 384), []
+    gru[1].gate[0] = torch.nn.Linear(384, 384, bias=False)
+    gru[1].res[0] = type("Same", (torch.nn.Linear,), {})(384, 384)
+    torch.nn.utils.parametrizations.weight_norm(gru[3].res[0])
+    gru[3].register_forward_hook(lambda m, a, y: seen.append(y))
+    y = gru(x)
+    h = gru[0](x)
+    h = gru[2](h + gru[1].gate(h) * gru[1].res(h))
+    torch.testing.assert_close(y, h + gru[3].gate(h) * gru[3].res(h))
+    assert len(seen) == 1 and seen[0] is y
+    g, = torch.autograd.grad(y.sum(), [gru[3].res[0].parametrizations.weight.original1])
+    assert g.abs().sum() > 0
