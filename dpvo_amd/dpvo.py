@@ -560,7 +560,8 @@ class DPVO:
             e_.record()                 # (creates the HIP event handle)
         dp = lambda t: t.data_ptr()
         upd = self.network.update
-        fp = (upd._packed or upd.pack())["_fparams"]
+        P = upd._packed or upd.pack()
+        fp = P["_fparams"]
         rings = ((self.pg.colors_, 0), (self.pg.poses_, 0), (self.pg.patches_, 0), (self.pg.intrinsics_, 0), (self.imap_, self.pmem),
                  (self._gmap_cl, self.pmem), (self._fmap1_cl, self.mem), (self._fmap2_cl, self.mem))
         hh, ww = self._fmap1_cl.shape[1:3]
@@ -593,7 +594,7 @@ class DPVO:
             a.P, a.pmem, a.mem, a.H0, a.W0 = self.P, self.pmem, self.mem, hh, ww
             a.H1, a.W1 = self._fmap2_cl.shape[1:3]
             a.patch_lifetime, a.ba_window, a.iterations, a.lmbda, a.mm_beta = cfg.PATCH_LIFETIME, cfg.OPTIMIZATION_WINDOW, 2, 1e-4, 0.5
-        fu["fparams"] = fp
+        fu["packed"] = P
         self._fu = fu
         return fu
 
@@ -618,7 +619,12 @@ class DPVO:
         kf.E, kf.n = E, n
         kf.forced = -1 if self.keyframe_override is None else int(bool(self.keyframe_override(self.counter)))
         upd = self.network.update
-        fu["fparams"].tiling, fu["fparams"].start_skew = upd.tiling, upd.start_skew
+        P = upd._packed or upd.pack()
+        if P is not fu["packed"]:               # packed anew since (another tracker with this network, a change of its parameters): the old images are gone
+            fu["packed"] = P
+            for b in fu["args"]:
+                b.upd = ctypes.addressof(P["_fparams"])
+        P["_fparams"].tiling, P["_fparams"].start_skew = upd.tiling, upd.start_skew
         a.net = es.a["net"].data_ptr()
         if es.net_pending is not None:
             a.net_rows, a.n_kept = es.net_pending[0].data_ptr(), es.net_pending[1]

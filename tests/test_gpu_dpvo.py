@@ -613,3 +613,40 @@ def test_plan_on_the_side_stream_is_bit_identical(dev):
         for k in ("ii", "jj", "kk", "net", "target", "weight"):
             assert torch.equal(getattr(a.pg, k), getattr(b.pg, k)), k
         assert torch.equal(a.pg.poses_[:a.n], b.pg.poses_[:b.n]) and torch.equal(a.pg.patches_[:a.n], b.pg.patches_[:b.n])
+
+
+def test_operand_images_packed_anew_while_tracking(dev):
+    """the one-call path follows the update operator's operand images: packed anew between two frames (a second tracker with this network does it), from
+    the same parameters the run stays the same bit for bit, and from others it uses those"""
+    def run(change):
+        cfg = base_cfg.clone(); cfg.merge_from_dict(DEFAULT_YAML)
+        cfg.PATCHES_PER_FRAME, cfg.BUFFER_SIZE = 16, 256
+        torch.manual_seed(5)
+        network = VONet()
+        slam = DPVO(cfg, network, ht=96, wd=128, device=dev, defer_keyframe=True, overlap_encoders=True)
+        slam.motion_probe = lambda: 1e9
+        slam.keyframe_override = lambda counter: False
+        g = torch.Generator().manual_seed(5)
+        intr = torch.tensor([100.0, 100.0, 64.0, 48.0], device=dev)
+        kept = []
+        for t in range(24):
+            if t == 16:
+                slam.flush()
+                assert slam._fu is not None, "the one-call path was not reached"
+                change(slam, network, cfg)
+                kept += [torch.full((384 * 896,), float("nan"), dtype=torch.float16, device=dev) for _ in range(64)]     # (over what was freed)
+            torch.manual_seed(t)
+            slam(float(t), torch.randint(0, 255, (3, 96, 128), generator=g, dtype=torch.uint8).to(dev), intr)
+        slam.flush()
+        torch.cuda.synchronize()
+        return slam.pg.net.clone(), slam.pg.poses_[:slam.n].clone()
+
+    def other(slam, network, cfg):
+        with torch.no_grad():
+            network.update.gru[3].res[2].weight.mul_(1.5)
+        network.update.pack()
+    plain = run(lambda *a: None)
+    for change in (lambda slam, network, cfg: network.update.pack(), lambda slam, network, cfg: DPVO(cfg, network, ht=96, wd=128, device=dev)):
+        assert all(torch.equal(a, b) for a, b in zip(plain, run(change)))
+    changed = run(other)
+    assert torch.isfinite(changed[0]).all() and not torch.equal(changed[0], plain[0])
