@@ -560,7 +560,7 @@ class DPVO:
             e_.record()                 # (creates the HIP event handle)
         dp = lambda t: t.data_ptr()
         upd = self.network.update
-        P = upd._packed or upd.pack()
+        P = upd.operands()
         fp = P["_fparams"]
         rings = ((self.pg.colors_, 0), (self.pg.poses_, 0), (self.pg.patches_, 0), (self.pg.intrinsics_, 0), (self.imap_, self.pmem),
                  (self._gmap_cl, self.pmem), (self._fmap1_cl, self.mem), (self._fmap2_cl, self.mem))
@@ -619,7 +619,7 @@ class DPVO:
         kf.E, kf.n = E, n
         kf.forced = -1 if self.keyframe_override is None else int(bool(self.keyframe_override(self.counter)))
         upd = self.network.update
-        P = upd._packed or upd.pack()
+        P = upd.operands()
         if P is not fu["packed"]:               # packed anew since (another tracker with this network, a change of its parameters): the old images are gone
             fu["packed"] = P
             for b in fu["args"]:

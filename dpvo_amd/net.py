@@ -147,10 +147,27 @@ def _read_all(seq, classes):
     return m
 
 
+class _Stage(nn.Module):
+    """a part of Update whose parameters may change without a mark on them (an optimiser's fused step leaves none): Update.operands() asks here"""
+    stale = 0                    # since Update's images were packed: 1 loaded, moved or cast; 2 a call was recorded for a backward pass
+
+    def _load_from_state_dict(self, *a, **k):
+        self.__dict__["stale"] = max(self.stale, 1)
+        return super()._load_from_state_dict(*a, **k)
+
+    def _apply(self, fn, *a, **k):
+        self.__dict__["stale"] = max(self.stale, 1)
+        return super()._apply(fn, *a, **k)
+
+    def _recorded(self, *parameters):
+        if torch.is_grad_enabled() and self.stale < 2 and any(p is not None and p.requires_grad for p in parameters):
+            self.__dict__["stale"] = 2
+
+
 _GATE, _RES = (nn.Linear, nn.Sigmoid), (nn.Linear, nn.ReLU, nn.Linear)
 
 
-class GatedResidual(nn.Module):
+class GatedResidual(_Stage):
     def __init__(self, dim):
         super().__init__()
         self.gate = nn.Sequential(nn.Linear(dim, dim), nn.Sigmoid())
@@ -161,20 +178,25 @@ class GatedResidual(nn.Module):
         The children's parameters are read (parametrized ones too), their calls do not happen: one with hooks or another forward is refused"""
         gate, _ = _read_all(self.gate, _GATE)
         first, _, last = _read_all(self.res, _RES)
-        to = lambda t: None if t is None else t.to(x.dtype)
-        return blocks.gated_residual(x, to(gate.weight), to(gate.bias), to(first.weight), to(first.bias), to(last.weight), to(last.bias))
+        par = gate.weight, gate.bias, first.weight, first.bias, last.weight, last.bias
+        self._recorded(*par)
+        return blocks.gated_residual(x, *(None if t is None else t.to(x.dtype) for t in par))
 
 
-class GatedStack(nn.Sequential):
+class GatedStack(_Stage, nn.Sequential):
     """LayerNorm, GatedResidual, LayerNorm, GatedResidual (net.py:44-49: Update.gru), differentiable: `update.gru(net)` trains or fine-tunes
-    this stage on its own.  The tracker does not come by here: Update.forward runs the stage inside its seven kernels."""
+    this stage on its own.  The tracker does not come by here: Update.forward runs the stage inside its seven kernels, from f16 images of the
+    parameters.  From the first recorded call of the stage on it packs them anew at every call; `update.pack()`, which a new tracker does by itself,
+    says that training is over."""
 
     def forward(self, x):
         for m in self:
             if isinstance(m, nn.LayerNorm):
                 if _read(m, nn.LayerNorm).normalized_shape != x.shape[-1:]:
                     raise L.DPVOHipError(f"{m} for rows of {tuple(x.shape[-1:])}")
-                x = blocks.norm(x, m.weight, m.bias, "layer", m.eps)
+                w, b = m.weight, m.bias
+                self._recorded(w, b)
+                x = blocks.norm(x, w, b, "layer", m.eps)
             else:
                 x = m(x)
         return x
@@ -215,8 +237,28 @@ class Update(nn.Module):
         self.start_skew = 0
 
     # -------------------------------------------------------------------------------------- operand images
+    def _stages(self):
+        gru = self._modules["gru"]
+        return [m for m in (gru, *gru._modules.values()) if "stale" in m.__dict__]      # (there once it is not 0)
+
     def pack(self):
-        """f16 weight images for the kernels (re-run after loading / changing parameters)."""
+        """f16 weight images for the kernels.  Loading, moving and casting parameters, and training `gru`, are followed by themselves (operands());
+        re-run it after any other change of them."""
+        for m in self._stages():
+            del m.__dict__["stale"]
+        return self._pack()
+
+    def operands(self):
+        """the images for a call: those at hand, or new ones where the parameters have changed, or may have (a stage that is being trained)"""
+        stages = self._stages()
+        if self._packed is not None and not stages:
+            return self._packed
+        for m in stages:
+            if m.stale < 2:
+                del m.__dict__["stale"]
+        return self._pack()
+
+    def _pack(self):
         h = lambda t: t.detach().to(torch.float16).contiguous()
         f = lambda t: t.detach().float().contiguous()
         dev = self.norm.weight.device
@@ -274,9 +316,9 @@ class Update(nn.Module):
         self._packed = None
         return super()._apply(fn, *a, **k)
 
-    def load_state_dict(self, *a, **k):
+    def _load_from_state_dict(self, *a, **k):            # (of a whole network's load too)
         self._packed = None
-        return super().load_state_dict(*a, **k)
+        return super()._load_from_state_dict(*a, **k)
 
     # -------------------------------------------------------------------------------------- forward
     @torch.no_grad()
@@ -293,7 +335,7 @@ class Update(nn.Module):
         removal whose compaction of `net` was deferred, EdgeStore.keep(defer_net=True)); the seven-launch kernels gather it in
         their first kernel, every other path gathers it here first.
         Returns net f32 [1,E,384], (delta f32 [1,E,2], weight f32 [1,E,2], None)."""
-        P = self._packed or self.pack()
+        P = self.operands()
         L.require_cuda(net, inp, corr, ii, jj, kk)
         E = ii.numel()
         dev = net.device

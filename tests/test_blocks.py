@@ -384,3 +384,60 @@ def test_children_that_are_read(monkeypatch):
     assert len(seen) == 1 and seen[0] is y
     g, = torch.autograd.grad(y.sum(), [gru[3].res[0].parametrizations.weight.original1])
     assert g.abs().sum() > 0
+
+
+def test_the_trackers_images_follow_training(monkeypatch):
+    """whatever changes the stage's parameters by way of its modules, the next call of the update operator has images of the new ones"""
+    from dpvo_amd import net as N
+    plain_blocks(monkeypatch)
+    torch.manual_seed(1)
+    network = N.VONet()
+    upd = network.update
+
+    def right():
+        fresh = N.Update(3)
+        fresh.load_state_dict(upd.state_dict(), assign=True)
+        P, want = upd.operands(), fresh.pack()
+        return all(torch.equal(a, b) for k in ("g0", "g1", "c1", "norm") for a, b in zip(P[k], want[k]))
+    upd.pack()
+    P = upd.operands()
+    assert upd.operands() is P and right()
+    with torch.no_grad():
+        upd.gru(z(1, 3, 384))
+    assert upd.operands() is P                                                  # nothing recorded: the images stay
+    opt = torch.optim.AdamW(upd.gru.parameters(), lr=0.1, fused=True)           # (leaves no mark on the parameters)
+    for use in ((), ("forward",), ("forward", "backward"), ("forward", "backward", "step")):    # after which of them the tracker runs too
+        y = upd.gru(torch.randn(1, 3, 384))
+        assert "forward" not in use or right()
+        y.square().sum().backward()
+        assert "backward" not in use or right()
+        opt.step()
+        assert right()
+    upd.pack()
+    P = upd.operands()
+    assert upd.operands() is P                                                  # training is over
+    for part in (upd.gru[1], upd.gru[3], upd.gru):                              # a part alone
+        part(torch.randn(1, 3, 384)).square().sum().backward()
+        assert right()
+        for p in part.parameters():
+            p.data.add_(0.01)
+        assert right()
+        upd.pack()
+    for n, p in upd.gru.named_parameters():                                     # the norms alone
+        p.requires_grad_(n.split(".")[0] in "02")
+    upd.gru(torch.randn(1, 3, 384)).sum().backward()
+    upd.gru[0].weight.data.add_(0.01)
+    assert right()
+    upd.pack()
+    for m in (network, upd, upd.gru, upd.gru[3]):                               # loads, casts
+        state = {k: torch.randn_like(v) if v.is_floating_point() else v for k, v in m.state_dict().items()}
+        for assign in (False, True):
+            P = upd.operands()
+            m.load_state_dict({k: v + assign for k, v in state.items()}, assign=assign)
+            assert upd.operands() is not P and right()
+            P = upd.operands()
+            assert upd.operands() is P
+        m.half()
+        assert upd.operands() is not P and right()
+        m.float()
+        assert right() and upd.operands() is upd.operands()

@@ -869,3 +869,34 @@ def test_pending_signs(dev, D):
         p, = torch.autograd.grad((run(*want) * dy).sum(), want[:1])
         q, = torch.autograd.grad((torch.complex(dy, run(*want)).conj().imag * -dy).sum(), want[:1])
         assert torch.equal(p, q), k
+
+
+def test_update_forward_after_training_the_stage(dev):
+    """Update.forward uses the parameters of the moment while `gru` is trained (f16, by a fused step)"""
+    from dpvo_amd import net as N
+    from tests import helpers as H
+    torch.manual_seed(6)
+    upd = N.Update(3).to(dev)
+    ii, jj, kk, _ = H.small_graph(14, 8)
+    E = ii.numel()
+    ii, jj, kk = ii.to(dev), jj.to(dev), kk.to(dev)
+    g = torch.Generator().manual_seed(0)
+    net, inp, corr = (torch.randn(1, E, n, generator=g).cuda() * s for n, s in ((384, 1.0), (384, 0.5), (882, 0.5)))
+    call = lambda u: u(net, inp.half(), corr.half(), None, ii, jj, kk)  # noqa: E731
+
+    def fresh():
+        u = N.Update(3).to(dev)
+        u.load_state_dict(upd.state_dict())
+        return u
+    first = call(upd)
+    opt = torch.optim.AdamW(upd.gru.parameters(), lr=0.05, fused=True)
+    for _ in range(2):
+        upd.gru(net.half()).float().square().mean().backward()
+        call(upd)
+        opt.step()
+        now, want = call(upd), call(fresh())
+        assert torch.equal(now[0], want[0]) and torch.equal(now[1][0], want[1][0]) and torch.equal(now[1][1], want[1][1])
+    assert not torch.equal(now[0], first[0])
+    upd.pack()
+    P = upd.operands()
+    assert upd.operands() is P and torch.equal(call(upd)[0], now[0])
