@@ -431,7 +431,8 @@ class _GatedResidual(torch.autograd.Function):
         with _on(x):
             dy = _rows(dy)[0]
             dg, dr = _dact(dy, g, r, _SIGMOID)
-            # the ReLU's derivative is where its output is positive: the gradient of its input is masked in the product's epilogue
+            # the ReLU's derivative is 0 where its output (as rounded: an f16 sum up to 2^-25 has become 0) is: the gradient of its input is masked in
+            # the product's epilogue, and a NaN passes
             dp = _dx([(dr, w2)], mask=t)[0] if need[0] or need[3] or need[4] else None
             if need[0]:
                 dx = _dx([(dg, wg), (dp, w1)], addend=dy)[0].view(x.shape)

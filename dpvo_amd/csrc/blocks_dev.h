@@ -125,7 +125,7 @@ enum { E_LIN = 0, E_GATE = 1, E_GATE2 = 2, E_DACT = 3 };
 // E_GATE  one A, two B: out0 = act(A.B0 + bias0) * (A.B1 + bias1) + addend (save0 / save1: the two sums in f32)
 // E_GATE2 the same with an A for each B
 // E_DACT  C is the gradient of h = act(save0) [* save1]: out0 = C [* save1] * act'(save0), out1 = C * act(save0) (with save1); with `mask`
-//         (h itself, act = relu) out0 = C where mask > 0
+//         (h itself, act = relu) out0 = C but where mask <= 0
 struct Prob {
   const void *A[2], *B[2];
   int64_t lda[2], ldb[2], K[2];

@@ -519,7 +519,7 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
                   load_n<T, 8>(extra + m * ldx + n, nv, t);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = EPI == E_DACT ? (t[e] > 0.f ? v[e] : 0.f) : v[e] + t[e];
+                for (int e = 0; e < 8; ++e) v[e] = EPI == E_DACT ? (t[e] <= 0.f ? 0.f : v[e]) : v[e] + t[e];   // (a NaN passes)
               }
               store_n<T, 8>((T*)P.out0 + m * P.ldo + n, nv, v);
             }

@@ -608,7 +608,7 @@ int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float* gate, cons
 
 /* Input gradient dx [M,N] = a0 b0 [+ a1 b1] [+ addend]: a_s [M,K_s] gradients of the sums, b_s [K_s,N] the weights as stored.
  * With `gate` (f32 [M,N] contiguous, as saved) dx is itself the gradient of act(gate) [* up] and is taken through it at once:
- * dx = d_gate, dx2 = d_up as in dpvo_gated_linear_dact; with `mask` [M,N] (the ReLU's output) dx is kept where mask > 0.
+ * dx = d_gate, dx2 = d_up as in dpvo_gated_linear_dact; with `mask` [M,N] (the ReLU's output) dx is 0 where mask <= 0 and kept elsewhere.
  * addend is allowed with neither.  ws: dpvo_gated_linear_dx_workspace_bytes(p) bytes (0: the sum is not cut into parts). */
 typedef struct {
   const void *a[2], *b[2], *addend, *mask;

@@ -900,3 +900,37 @@ def test_update_forward_after_training_the_stage(dev):
     upd.pack()
     P = upd.operands()
     assert upd.operands() is P and torch.equal(call(upd)[0], now[0])
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,D,H", [(3, 70, 40), (100, 70, 40), (300, 200, 150), (5000, 384, 385)])
+def test_nan_shows_in_gradients_of_the_gated_residual(dev, t, M, D, H):
+    """a NaN in a row, or in a hidden bias, reaches the gradients that it makes unknown -- the ReLU's mask does not turn it into a 0 -- and no others"""
+    g = torch.Generator().manual_seed(M)
+    x = make(g, M, D, t=t)
+    wg, bg = layer(g, D, D, t)
+    w1, b1 = layer(g, H, D, t)
+    w2, b2 = layer(g, D, H, t)
+    dy = make(g, M, D, t=t, grad=False)
+    leaves = [x, wg, bg, w1, b1, w2, b2]
+    d0 = torch.autograd.grad(blocks.gated_residual(*leaves), leaves, dy)
+    with torch.no_grad():
+        bad = [p.clone() for p in leaves]
+        bad[0][1, 5] = float("nan")
+    bad = [p.requires_grad_() for p in bad]
+    y = blocks.gated_residual(*bad)
+    d1 = torch.autograd.grad(y, bad, dy)
+    keep = [i for i in range(M) if i != 1]
+    assert y[1].isnan().all() and y[keep].isfinite().all()
+    assert d1[0][1].isnan().all() and torch.equal(d1[0][keep], d0[0][keep])
+    for got in d1[1:]:                                                          # every weight and bias sums over the bad row
+        assert got.isnan().all()
+    with torch.no_grad():
+        bad = [p.clone() for p in leaves]
+        bad[4][7] = float("nan")                                                # one hidden feature: of no row's gate, of every row's product
+    bad = [p.requires_grad_() for p in bad]
+    d1 = torch.autograd.grad(blocks.gated_residual(*bad), bad, dy)
+    rows = [i for i in range(H) if i != 7]
+    # the hidden layer's gradient is known but for that feature, where the formula has a NaN's derivative times a number
+    assert torch.equal(d1[4][rows], d0[4][rows]) and torch.equal(d1[3][rows], d0[3][rows])
+    assert torch.equal(d1[5][:, rows], d0[5][:, rows]) and d1[5][:, 7].isnan().all()
