@@ -72,7 +72,7 @@ template <bool FINE> __device__ __forceinline__ float act_(int a, float z) {
 struct ActD { float y, d; };
 template <bool FINE> __device__ __forceinline__ ActD act_d(int a, float z) {
   switch (a) {
-    case DPVO_ACT_RELU: return {z < 0.f ? 0.f : z, z > 0.f ? 1.f : 0.f};
+    case DPVO_ACT_RELU: return {z < 0.f ? 0.f : z, z <= 0.f ? 0.f : 1.f};          // (of a NaN as of a sum that may be positive: nothing is hidden)
     case DPVO_ACT_SIGMOID: { const float s = sigmoid_<FINE>(z); return {s, s * (1.f - s)}; }
     case DPVO_ACT_SILU: { const float s = sigmoid_<FINE>(z); return {z * s, s + z * (s * (1.f - s))}; }
     case DPVO_ACT_GELU: {

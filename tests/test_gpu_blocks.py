@@ -934,3 +934,29 @@ def test_nan_shows_in_gradients_of_the_gated_residual(dev, t, M, D, H):
     # the hidden layer's gradient is known but for that feature, where the formula has a NaN's derivative times a number
     assert torch.equal(d1[4][rows], d0[4][rows]) and torch.equal(d1[3][rows], d0[3][rows])
     assert torch.equal(d1[5][:, rows], d0[5][:, rows]) and d1[5][:, 7].isnan().all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N", [(3, 20, 7), (200, 72, 90), (3000, 200, 130)])
+def test_nan_passes_the_relus_derivative(dev, t, M, K, N):
+    """relu of a NaN sum: the gradient that arrives goes on (as by a mask of `<= 0`), so that its bias and weights do not look clean"""
+    g = torch.Generator().manual_seed(M)
+    x, dy = make(g, M, K, t=t, grad=False), make(g, M, N, t=t, grad=False)
+    w, b = layer(g, N, K, t)
+    wu, _ = layer(g, N, K, t, False)
+    with torch.no_grad():
+        b[2] = float("nan")
+    db, = torch.autograd.grad(blocks.linear(x, w, b, "relu"), b, dy)
+    within(db[2:3], rows_f(dy[:, 2:3]).sum0(), t, "db")
+    dw, db = torch.autograd.grad(blocks.gated_linear(x, w, wu, b, activation="relu"), (w, b), dy)
+    U_ = proj(rows_f(x), rows_f(wu))
+    d = rows_f(dy[:, 2:3]) * V(U_.v[:, 2:3], U_.e[:, 2:3])
+    within(db[2:3], d.to(t).sum0(), t, "db gated")
+    within(dw[2:3], d.to(t).t().mm(rows_f(x)), t, "dw gated")
+    h, gate = make(g, M, N, t=t, grad=False), make(g, M, N, t=t, grad=False)
+    gate[1, 3] = float("nan")
+    gate.requires_grad_()
+    s, _ = blocks.residual_norm(torch.zeros_like(h), h, norm=None, gate=gate, gate_activation="relu")
+    got, = torch.autograd.grad(s, gate, dy)
+    want = dy * h * (gate.detach() <= 0).logical_not()
+    assert s[1, 3].isnan() and torch.equal(got, want)
