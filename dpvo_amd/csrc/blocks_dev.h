@@ -80,8 +80,9 @@ template <bool FINE> __device__ __forceinline__ ActD act_d(int a, float z) {
       return {z * c, c + z * (0.39894228040143268f * exp_<FINE>(-0.5f * z * z))};
     }
     case DPVO_ACT_GELU_TANH: {
-      const float t = tanh_<FINE>(0.79788456080286536f * (z + 0.044715f * z * z * z));
-      return {0.5f * z * (1.f + t), 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * (0.79788456080286536f * (1.f + 0.134145f * z * z))};
+      const float t = tanh_<FINE>(0.79788456080286536f * (z + 0.044715f * z * z * z)), r = 1.f - t * t;
+      // (r is 0 from |z| of some 5 on; z * z is infinite from 2^64 on, and the product would be a NaN)
+      return {0.5f * z * (1.f + t), 0.5f * (1.f + t) + (r == 0.f ? 0.f : 0.5f * z * r * (0.79788456080286536f * (1.f + 0.134145f * z * z)))};
     }
     default: return {z, 1.f};
   }

@@ -960,3 +960,25 @@ def test_nan_passes_the_relus_derivative(dev, t, M, K, N):
     got, = torch.autograd.grad(s, gate, dy)
     want = dy * h * (gate.detach() <= 0).logical_not()
     assert s[1, 3].isnan() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("t", [BF16, F32], ids=str)
+@pytest.mark.parametrize("a", list(blocks.ACTIVATIONS))
+def test_derivatives_at_large_sums(dev, t, a):
+    """sums of 1 to 2^120, of either sign, one to a row: far from 0 every derivative is 0 or 1 (the identity's: 1; the sigmoid's: 0)"""
+    z = torch.tensor([s * 2.0 ** e for e in range(0, 121) for s in (1, -1)])[:, None].to(t).cuda()
+    one = torch.ones(1, 1, dtype=t, device=dev)
+    x = z.clone().requires_grad_()
+    u = torch.ones_like(z).requires_grad_()
+    Z = rows_f(z)
+    v, d = act(a, Z)
+    # (values of the 64-bit form where its own powers overflow: x^3 does not before 2^341)
+    y = blocks.linear(x, one, None, a)
+    within(y, v, t, "y")
+    got, = torch.autograd.grad(y, x, torch.ones_like(y))
+    # |z| >= 2^20: `act`'s bound of the derivative grows with |z|, the derivative does not
+    far = (Z.v.abs() >= 2.0 ** 20).flatten()
+    within(got[~far], V(d.v[~far], d.e[~far]), t, "dx")
+    assert torch.equal(got[far].double().cpu(), d.v[far]), got[far].flatten()
+    gx, gu = torch.autograd.grad(blocks.gated_linear(x, one, one, activation=a, up_input=u), (x, u), torch.ones_like(y))
+    assert torch.equal(gx, got) and torch.equal(gu, y)
