@@ -48,8 +48,8 @@ template <class T, int N> __device__ __forceinline__ void store_n(T* p, int nv, 
   }
 }
 
-// ---- activations.  FINE: expf / tanhf / division (f32 operands); otherwise the hardware exponential and reciprocal, whose error (a few
-// 2^-22) is far below the half step of a 16-bit result (2^-11 / 2^-8).
+// ---- activations.  FINE: expf / tanhf / division, for f32 results (f32 operands, and a 16-bit gate beside an f32 stream); otherwise the hardware
+// exponential and reciprocal, whose error (2^-23 of |z| and a few 2^-22) is far below the half step of a 16-bit result (2^-11 / 2^-8).
 template <bool FINE> __device__ __forceinline__ float exp_(float x) { return FINE ? expf(x) : __expf(x); }
 template <bool FINE> __device__ __forceinline__ float rcp_(float x) { return FINE ? 1.f / x : __builtin_amdgcn_rcpf(x); }
 template <bool FINE> __device__ __forceinline__ float sigmoid_(float x) { return rcp_<FINE>(1.f + exp_<FINE>(-x)); }

@@ -269,7 +269,7 @@ template <class NX, class NB, int L, bool RAGGED> __global__ void __launch_bound
         for (int e = 0; e < P; ++e) f[e] = f[e] * pw[e] + pb[e];
       }
       if (p.gate) {
-        act_n<sizeof(NB) == 4, false, P>(p.gate_activation, g);
+        act_n<sizeof(NX) == 4, false, P>(p.gate_activation, g);
 #pragma unroll
         for (int e = 0; e < P; ++e) s[e] += p.scale * (g[e] * f[e]);
       } else {
@@ -409,7 +409,7 @@ template <class NX, class NB, int L, bool RAGGED> __global__ void __launch_bound
           for (int e = 0; e < P; ++e) t[e] = f[e];
         }
         if (p.gate) {
-          act_d_n<sizeof(NB) == 4, false, P>(p.gate_activation, gd, ga);
+          act_d_n<sizeof(NX) == 4, false, P>(p.gate_activation, gd, ga);
         } else {
 #pragma unroll
           for (int e = 0; e < P; ++e) {
@@ -509,7 +509,7 @@ template <class NX, class NB, int L, int V, bool RAGGED> __global__ void __launc
         wide_post(row, p, i, f + i * E, t);
         if (p.gate) {
           row.piece((const NB*)p.gate + (int64_t)((uint32_t)m / a.rows_per_gate) * p.ldgate, i, u);
-          act_n<sizeof(NB) == 4, false, E>(p.gate_activation, u);
+          act_n<sizeof(NX) == 4, false, E>(p.gate_activation, u);
 #pragma unroll
           for (int e = 0; e < E; ++e) t[e] *= u[e];
         }
@@ -566,7 +566,7 @@ template <class NX, class NB, int L, int V, bool RAGGED> __global__ void __launc
           wide_post(row, p, i, f + i * E, t);
           if (gate) {
             row.piece(gate, i, u);
-            act_n<sizeof(NB) == 4, false, E>(p.gate_activation, u);
+            act_n<sizeof(NX) == 4, false, E>(p.gate_activation, u);
 #pragma unroll
             for (int e = 0; e < E; ++e) t[e] *= u[e];
           }
@@ -612,7 +612,7 @@ template <class NX, class NB, int L, int V, bool RAGGED> __global__ void __launc
       if (gate) {
         float t[E], u[E], y[E];
         row.piece(gate, i, u);
-        act_d_n<sizeof(NB) == 4, false, E>(p.gate_activation, u, y);
+        act_d_n<sizeof(NX) == 4, false, E>(p.gate_activation, u, y);
         if (p.dgate && !a.part_gate) {
           wide_post(row, p, i, f + i * E, t);
 #pragma unroll
@@ -692,7 +692,7 @@ template <class NX, class NB> __global__ void __launch_bounds__(256, 2) norm_col
           t[e] = post ? f[e] * pw[e] + pb[e] : f[e];
         }
         if (p.gate) {
-          act_d_n<sizeof(NB) == 4, false, E>(p.gate_activation, gd, ga);
+          act_d_n<sizeof(NX) == 4, false, E>(p.gate_activation, gd, ga);
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e) ga[e] = 1.f, gd[e] = 0.f;

@@ -982,3 +982,19 @@ def test_derivatives_at_large_sums(dev, t, a):
     assert torch.equal(got[far].double().cpu(), d.v[far]), got[far].flatten()
     gx, gu = torch.autograd.grad(blocks.gated_linear(x, one, one, activation=a, up_input=u), (x, u), torch.ones_like(y))
     assert torch.equal(gx, got) and torch.equal(gu, y)
+
+
+@pytest.mark.parametrize("tb", [F16, BF16, F32], ids=str)
+@pytest.mark.parametrize("a,D", [("sigmoid", 384), ("silu", 384), ("sigmoid", 385), ("silu", 4000), ("sigmoid", 4104), ("silu", 5001)])
+def test_gates_of_a_f32_stream_are_f32(dev, tb, a, D):
+    """act(gate) where it is itself the f32 result (0 + gate * 1), and where it is a f32 gradient (of post_bias, over one row): 1 / (1 + e) from an
+    exponential within a unit in the last place (2 U of e / (1 + e)), a sum and a division (U each), and silu's or the gradient's product (U): 5 U"""
+    gate = torch.linspace(-20, 20, D).to(tb).cuda()
+    v = act(a, rows_f(gate))[0].v
+    x, one = torch.zeros(1, D, device=dev), torch.ones(1, D, dtype=tb, device=dev)
+    s, _ = blocks.residual_norm(x, one, norm=None, gate=gate, gate_activation=a)
+    within(s[0], V(v, 5 * U * v.abs()), F32, "s")
+    pw, pb = torch.ones(D, device=dev), torch.zeros(D, device=dev, requires_grad=True)
+    s, _ = blocks.residual_norm(x, one, norm=None, gate=gate, gate_activation=a, post_norm="rms", post_weight=pw, post_bias=pb)
+    got, = torch.autograd.grad(s, pb, torch.ones_like(s))
+    within(got, V(v, 5 * U * v.abs()), F32, "d post_bias")
