@@ -700,8 +700,9 @@ template <int FORM, int EPI, int KIND> int go(const GemmArgs& a, int64_t tiles, 
 int BLK_ENTRY(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s) {
   if (tiles == 0) return DPVO_OK;
   if (kind == T_FEW) return epi == E_LIN ? few<E_LIN>(a, tiles, s) : epi == E_GATE ? few<E_GATE>(a, tiles, s) : few<E_GATE2>(a, tiles, s);
+  // (256 x 256 is never chosen for f32, nor for two inputs: not built)
 #define BLK_GO(F, E) if (form == F && epi == E) switch (kind) { \
-    case T_BIG: return E == E_GATE2 ? DPVO_E_UNSUPPORTED : go<F, E, E == E_GATE2 ? T_TILE : T_BIG>(a, tiles, s); \
+    case T_BIG: if constexpr (sizeof(T) == 2 && E != E_GATE2) return go<F, E, T_BIG>(a, tiles, s); else return DPVO_E_UNSUPPORTED; \
     case T_SMALL: return go<F, E, T_SMALL>(a, tiles, s); \
     case T_TINY: return go<F, E, T_TINY>(a, tiles, s); \
     default: return go<F, E, T_TILE>(a, tiles, s); }
