@@ -7,19 +7,12 @@
 namespace blk {
 namespace {
 
-inline bool type_ok(int t) { return t == DPVO_F16 || t == DPVO_BF16 || t == DPVO_F32; }
-inline int type_size(int t) { return t == DPVO_F32 ? 4 : 2; }
-inline bool act_ok(int a) { return a >= DPVO_ACT_IDENTITY && a <= DPVO_ACT_GELU_TANH; }
-// row offsets within a tile are 32-bit bytes
-inline bool ld_ok(int64_t ld, int64_t width, int size) { return ld >= width && ld <= INT_MAX / (256 * size); }
-
 int gemm(const GemmArgs& a, int dtype, int form, int epi, int kind, int64_t tiles, hipStream_t s) {
   if (tiles > INT_MAX) return DPVO_E_UNSUPPORTED;
   if (dtype == DPVO_F16) return gemm_f16(a, form, epi, kind, tiles, s);
   if (dtype == DPVO_BF16) return gemm_bf16(a, form, epi, kind, tiles, s);
   return gemm_f32(a, form, epi, kind, tiles, s);
 }
-inline int block_k(int dtype) { return dtype == DPVO_F32 ? 32 : 64; }
 
 // out[e] = sum over parts of part[i][e] (+ bias[e % N]) (+ addend[e]), all contiguous; a job for each row of the grid
 struct SumJob {
@@ -156,39 +149,6 @@ int col_reduce(const ColArgs& c, hipStream_t s) {
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
-// ---- which tiles, and in how many parts the summed index is cut where there are too few of them
-struct Plan {
-  int kind;
-  int64_t splits;
-};
-inline int tile_size(int kind) { return kind == T_BIG ? 256 : kind == T_SMALL || kind == T_TINY ? 64 : 128; }
-// `count(t)`: tiles of t x t; nb: blocks of the summed index; cut: whether parts are possible.
-//  - 256 x 256 reads LDS least per product and gives 1127 Tflop/s (bf16, 8192 x 8192 x 4096: 488 us) where 128 x 128 gives 897 (613 us), so a round
-//    of the latter (two workgroups on each of 256 compute units) takes 0.62 of a round of the former (one): whichever needs less.  But nothing
-//    hides the epilogue of one workgroup alone: with 16 blocks it still wins (73.2 against 86.0 us, 4096 x 4096 x 1024 twice), with 6 it loses
-//    (55.8 against 49.5 us, 45312 x 384 x 384 twice); f32 products are bound by the matrix unit and gain nothing.
-//  - 128 x 128 wants its two workgroups: at 432 tiles it wins over 64 x 64 (16.6 against 20.4 us, 9216 x 768 x 384), at 256 it loses (20.7 against
-//    18.7, 2048 x 2048 x 1024).
-//  - Parts: towards two workgroups a compute unit, each with 12 blocks at least (a part costs a tile's write and read in f32, and all of them a
-//    launch); dw 384 x 384 over 45312 rows: 45 us in 56 parts, 56 in 64, 59 in 16.  Where that does not fill them, small tiles in parts of 4
-//    blocks at least: over 9216 rows 23 us in 21 parts, 25 with large tiles in 16.  Below 16 blocks a second launch costs more than it
-//    saves: 333 x 2048 x 768 8.6 us whole, 14.0 in three.
-//  - 64 x 64 by four waves where there are few: 1237 x 385 x 882 in f32 24.6 us against 40.5 with two waves, at 864 tiles 13.3 against 11.6.
-template <class F> Plan plan(F count, int64_t nb, int dtype, bool cut) {
-  const int64_t t = count(128);
-  if (dtype != DPVO_F32 && nb >= 16 && cdiv64(count(256), 256) * 100 < cdiv64(t, 512) * 62) return {T_BIG, 1};
-  if (t >= 384) return {T_TILE, 1};
-  const int small = count(64) >= 640 ? T_SMALL : T_TINY;
-  if (!cut || t == 0 || nb < 16) return {small, 1};
-  auto parts = [&](int64_t want, int64_t least) {
-    const int64_t n = want < nb / least ? want : nb / least;
-    return n < 1 ? 1 : n > 64 ? 64 : n;
-  };
-  const int64_t n = parts(512 / t, 12);
-  if (n * t >= 384) return {T_TILE, n};
-  return {small, parts(768 / count(64), 4)};
-}
-inline int64_t tiles(int64_t M, int64_t N, int t) { return cdiv64(M, t) * cdiv64(N, t); }
 int64_t tiles_of(Prob& p, int kind, int halves = 1) {
   const int t = tile_size(kind);
   p.tm = cdiv64(p.M, t);
@@ -196,33 +156,6 @@ int64_t tiles_of(Prob& p, int kind, int halves = 1) {
   return p.tm * p.tn;
 }
 
-// ---- the norm backward's share of rows
-struct NormPlan {
-  int sh;
-  int64_t groups, rpg, gpb, bpg, blocks;
-  bool shared;                                           // gate rows that several rows share
-};
-NormPlan norm_plan(const dpvo_residual_norm_t& p) {
-  NormPlan n;
-  n.shared = p.f && p.gate && p.groups < p.M;
-  n.sh = norm_shape(p, true, norm_sums(p, n.shared));
-  n.groups = n.shared ? p.groups : 1;
-  n.rpg = n.groups ? p.M / n.groups : 0;
-  // 4096 waves, four to a SIMD: enough loads in flight for the memory, few enough that their partial rows stay a few per cent of the traffic
-  const int L = n.sh == NORM_WIDE ? 0 : NORM_SHAPES[n.sh].L;
-  // (wide rows: rows of 2048 columns' sums, two to four workgroups a compute unit; 4096 x 8192 bf16 221 us in 64 parts, 130 in 128, 138 in 256)
-  const int64_t want = n.sh == NORM_WIDE ? 128 : L > 64 ? 4096 / (L / 64) : 1024, rounds = cdiv64(n.rpg, norm_slots(n.sh));
-  if (n.groups >= want) {
-    n.bpg = 1;
-    n.gpb = cdiv64(n.groups, want);
-  } else {
-    n.gpb = 1;
-    n.bpg = n.groups ? want / n.groups : 1;
-    if (n.bpg > rounds) n.bpg = rounds < 1 ? 1 : rounds;
-  }
-  n.blocks = cdiv64(n.groups, n.gpb) * n.bpg;
-  return n;
-}
 int norm_check(const dpvo_residual_norm_t* p) {
   if (!p || p->M < 0 || p->D < 1 || !type_ok(p->x_dtype) || !type_ok(p->f_dtype) || !type_ok(p->w_dtype)) return DPVO_E_INVALID;
   if (p->x_dtype != p->f_dtype && p->x_dtype != DPVO_F32) return DPVO_E_UNSUPPORTED;
@@ -245,35 +178,6 @@ int norm_run(const NormArgs& a, int sh, bool back, int64_t blocks, hipStream_t s
 }  // namespace blk
 
 using namespace blk;
-
-// A plain projection (no activation, nothing saved) may be cut into parts like a gradient's sum
-static bool linear_cut(const dpvo_gated_linear_t* p) {
-  return !p->w_up && p->activation == DPVO_ACT_IDENTITY && !p->save_gate && p->ldy == p->N && (!p->residual || p->ldr == p->N);
-}
-static Plan linear_plan(const dpvo_gated_linear_t* p, int epi) {
-  const int bk = block_k(p->dtype);
-  Plan c = plan([&](int t) { return tiles(p->M, epi == E_GATE ? 2 * p->N : p->N, t); }, cdiv64(p->K, bk) + (epi == E_GATE2 ? cdiv64(p->Kv, bk) : 0),
-                p->dtype, linear_cut(p));
-  if (epi == E_GATE2 && c.kind == T_BIG) c.kind = T_TILE;      // (two sets of sums do not fit the registers of the largest tile)
-  return c;
-}
-// The few-row kernel's workgroups (64 rows x 16 columns) instead of tiles: up to 16 rows, and wherever they are one to a compute unit at most (f16
-// 200 x 1024 x 1024 relu 7.5 against 10.3 us, with 384 of them 12.7 against 10.5); twice as many up to 32 rows, where half of their products are
-// for nothing but the weights' bytes count, and for two inputs in f32 (200 x 384 x 384 10.7 against 24.2 us, with 384 of them 18.6 against
-// 24.3, with 768 28.1 against 25.0).  Beyond 16 rows not
-//  - for 16-bit rows of odd length, whose unaligned pieces the tiles load once and these workgroups again and again (96 x 882 x 385: 14.9 against
-//    9.0 us, with 386 columns 7.7 against 8.1; by the length and not the address, so that a result does not depend on where its operands lie),
-//  - for long sums that may be cut into parts (f16 96 x 1024 x 4096: 20.1 against 14.8 us, 96 x 768 x 2048 11.5 against 11.8).
-static bool linear_few(const dpvo_gated_linear_t* p, int epi) {
-  if (p->M <= 16) return true;
-  if (cdiv64(p->N, 16) * cdiv64(p->M, 64) > (p->M <= 32 || (epi == E_GATE2 && p->dtype == DPVO_F32) ? 512 : 256)) return false;
-  if (p->dtype != DPVO_F32 && (p->K % 2 || (p->w_up && p->Kv % 2))) return false;
-  return !(linear_cut(p) && p->K > 2048);
-}
-static int linear_epi(const dpvo_gated_linear_t* p) {
-  if (!p->w_up) return E_LIN;
-  return p->v == p->x && p->ldv == p->ldx && p->Kv == p->K ? E_GATE : E_GATE2;
-}
 
 extern "C" size_t dpvo_gated_linear_workspace_bytes(const dpvo_gated_linear_t* p) {
   if (!p || !type_ok(p->dtype) || p->M <= 0 || p->N <= 0 || p->K < 0 || p->Kv < 0 || p->w_up) return 0;
@@ -330,8 +234,6 @@ extern "C" int dpvo_gated_linear_dact(const void* dy, int64_t lddy, const float*
   DPVO_LAUNCH_CHECK();
   return DPVO_OK;
 }
-
-static Plan dx_plan(int64_t M, int64_t N, int64_t nb, int dtype, bool cut) { return plan([&](int t) { return tiles(M, N, t); }, nb, dtype, cut); }
 
 extern "C" size_t dpvo_gated_linear_dx_workspace_bytes(const dpvo_gated_linear_dx_t* p) {
   if (!p || !type_ok(p->dtype) || p->M <= 0 || p->N <= 0 || p->K[0] < 0 || p->K[1] < 0 || p->gate || p->mask) return 0;
@@ -393,14 +295,6 @@ extern "C" int dpvo_gated_linear_dx(const dpvo_gated_linear_dx_t* p, void* ws, s
 }
 
 // workspace: the parts of each product and of its column sums
-static Plan dw_plan(const dpvo_gated_linear_dw_t* p) {
-  return plan([&](int t) {
-    int64_t n = 0;
-    for (int i = 0; i < p->n; ++i)
-      n += tiles(p->N[i], p->K[i], t);
-    return n;
-  }, cdiv64(p->M, block_k(p->dtype)), p->dtype, true);
-}
 static bool dw_ok(const dpvo_gated_linear_dw_t* p) {
   if (!p || p->n < 0 || p->n > MAXP || !type_ok(p->dtype) || p->M < 0) return false;
   for (int i = 0; i < p->n; ++i) {

@@ -2,6 +2,7 @@
 // types, loads and stores that end at a row's end, the activations and their derivatives.  Sums, statistics and activations are f32 throughout.
 #pragma once
 #include "common.h"
+#include "blocks_plan.h"
 
 #define BLK_INLINE __attribute__((always_inline))      // for lambdas: one that stays a call keeps its captures in scratch
 
@@ -120,8 +121,6 @@ template <bool FINE, bool ALL, int N> __device__ __forceinline__ void act_d_n(in
 
 // ---- the matrix products' arguments.  C[M,N] = sum over segments s of A_s . B_s, where an operand is stored either with the summed index
 // contiguous ("row": A [M,K], B [N,K]) or with it as the row ("col": A [K,M], B [K,N]).
-enum { F_NT = 0, F_NN = 1, F_TN = 2 };                  // (A row, B row) forward; (A row, B col) input gradients; (A col, B col) weight gradients
-enum { E_LIN = 0, E_GATE = 1, E_GATE2 = 2, E_DACT = 3 };
 // E_LIN   out0 = act(C + bias0) + addend (save0: C + bias0 in f32); or, with `part`, the bare sum of this split in f32
 // E_GATE  one A, two B: out0 = act(A.B0 + bias0) * (A.B1 + bias1) + addend (save0 / save1: the two sums in f32)
 // E_GATE2 the same with an A for each B
@@ -141,14 +140,10 @@ struct Prob {
   int64_t nb0, nb;                                       // blocks of the summed index: first segment, all
   int splits, act;
 };
-constexpr int MAXP = 4;
 struct GemmArgs {
   Prob p[MAXP];
   int n;
 };
-
-// how a product is run: tiles of 128 x 128, 256 x 256 or 64 x 64 (by two waves or four), or few rows with the summed index over the waves (blocks_gemm.h)
-enum { T_TILE = 0, T_BIG = 1, T_SMALL = 2, T_TINY = 3, T_FEW = 4 };
 
 int gemm_f16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);
 int gemm_bf16(const GemmArgs& a, int form, int epi, int kind, int64_t tiles, hipStream_t s);

@@ -30,25 +30,6 @@ struct NormArgs {
 };
 constexpr int NORM_STATS = 6;
 
-// How a row of D elements is spread: 8 on each of L lanes, which keeps the backward's arrays of them in registers.  Four or more rows share
-// a workgroup where L <= 64 (no barriers there).  RAGGED: D is no multiple of 8.  Rows of more than 4096 elements go to the wide kernels, except
-// that the backward of 16-bit ones of up to 8192, in whole pieces and with up to four sums in LDS, still fits 1024 lanes (4096 x 8192: 153 us, wide
-// 254; f32 streams spill there: 884 us, wide 350; the forward takes 73 and 76 us, at 4096 x 5120 82 and 74).
-struct NormShape { int L; bool ragged; };
-constexpr NormShape NORM_SHAPES[] = {{16, false}, {32, false}, {64, false}, {128, false}, {256, false}, {512, false},
-                                     {16, true}, {32, true}, {64, true}, {128, true}, {256, true}, {512, true}, {1024, false}};
-constexpr int NORM_1024 = 12, NORM_WIDE = 13, NORM_MAX_D = 16384;
-inline int norm_sums(const dpvo_residual_norm_t& p, bool shared) {
-  return (p.dw != nullptr) + (p.db != nullptr) + (p.dpw != nullptr) + (p.dpb != nullptr) + (shared && p.dgate);
-}
-inline int norm_shape(const dpvo_residual_norm_t& p, bool back, int sums) {
-  if (p.D > 512 * 8) return back && p.D <= 1024 * 8 && p.D % 8 == 0 && p.x_dtype != DPVO_F32 && sums <= 4 ? NORM_1024 : NORM_WIDE;
-  int i = p.D % 8 ? 6 : 0;
-  while (NORM_SHAPES[i].L * 8 < p.D) ++i;
-  return i;
-}
-inline int norm_slots(int shape) { return shape == NORM_WIDE || NORM_SHAPES[shape].L > 64 ? 1 : 256 / NORM_SHAPES[shape].L; }   // rows at a time in a workgroup
-
 int norm_f16(const NormArgs& a, int shape, bool back, int64_t blocks, hipStream_t st);     // branch types; stream: the same or f32
 int norm_bf16(const NormArgs& a, int shape, bool back, int64_t blocks, hipStream_t st);
 int norm_f32(const NormArgs& a, int shape, bool back, int64_t blocks, hipStream_t st);
