@@ -441,3 +441,156 @@ def test_the_trackers_images_follow_training(monkeypatch):
         assert upd.operands() is not P and right()
         m.float()
         assert right() and upd.operands() is upd.operands()
+
+
+# ------------------------------------------------------------------------------------------------------------------ what the GPU tests reach
+PATHS = r"""
+#include <stdio.h>
+#include <string.h>
+#include <set>
+#include <string>
+#include "blocks_plan.h"
+using namespace blk;
+static std::string key(int form, int epi, int dtype, Plan c) {
+  static const char *forms[] = {"nt", "nn", "tn"}, *epis[] = {"lin", "gate", "gate2", "dact"}, *kinds[] = {"tile", "big", "small", "tiny", "few"};
+  return std::string(dtype == DPVO_F32 ? "f32 " : "16 ") + forms[form] + " " + epis[epi] + " " + kinds[c.kind] + (c.splits > 1 ? " parts" : "");
+}
+// y [M,N] from x [M,K]; inputs: 0 without a second product, 1 and 2; plain: no activation, nothing saved
+static std::string forward(int dtype, int inputs, bool plain, int64_t M, int64_t K, int64_t N) {
+  char x[2];
+  float save;
+  dpvo_gated_linear_t p = {};
+  p.x = x, p.v = inputs == 2 ? x + 1 : x, p.w_gate = x, p.w_up = inputs ? x : nullptr, p.save_gate = plain ? nullptr : &save;
+  p.ldx = p.ldwg = p.ldv = p.ldwu = p.K = K, p.Kv = inputs ? K : 0, p.ldy = p.N = N, p.M = M, p.dtype = dtype, p.activation = !plain;
+  const int e = linear_epi(&p);
+  if (!linear_few(&p, e)) return key(F_NT, e, dtype, linear_plan(&p, e));
+  return key(F_NT, e, dtype, Plan{T_FEW, 1}) + (M > 16 ? " 64 rows" : K > (dtype == DPVO_F32 ? 512 : 1024) ? " 16 waves" : " 4 waves");
+}
+static std::string dx(int dtype, bool through, int64_t M, int64_t N, int64_t nb) { return key(F_NN, through ? E_DACT : E_LIN, dtype, dx_plan(M, N, nb, dtype, !through)); }
+int main() {
+  std::set<std::string> all;
+  const int64_t size[] = {1, 7, 16, 17, 33, 64, 100, 200, 300, 500, 700, 1000, 1500, 2000, 4100, 6000, 9000, 20000, 45000}, sum[] = {7, 64, 200, 384, 500, 700, 1024, 1100, 2100, 4200, 9000};
+  for (int t = 0; t < 3; ++t)
+    for (int64_t M : size)
+      for (int64_t N : size)
+        for (int64_t K : sum) {
+          all.insert(forward(t, 0, true, M, K, N));
+          for (int i = 0; i < 3; ++i) all.insert(forward(t, i, false, M, K, N));
+          const int64_t nb = ceil_div(K, block_k(t));
+          all.insert(dx(t, false, M, N, nb)), all.insert(dx(t, false, M, N, 2 * nb)), all.insert(dx(t, true, M, N, nb));
+          for (int n = 1; n <= MAXP; ++n)
+            for (int sides = 0; sides < 2; ++sides) {
+              dpvo_gated_linear_dw_t p = {};
+              p.n = n, p.M = sides ? K * 5 : M, p.dtype = t;
+              for (int i = 0; i < n; ++i) p.N[i] = N, p.K[i] = sides ? M : K;
+              all.insert(key(F_TN, E_LIN, t, dw_plan(&p)));
+            }
+        }
+  for (auto& k : all) printf("all %s\n", k.c_str());
+  char op[16];
+  while (scanf("%15s", op) == 1) {
+    long a[32];
+    int n;
+    if (scanf("%d", &n) != 1 || n > 32) return 1;
+    for (int i = 0; i < n; ++i)
+      if (scanf("%ld", a + i) != 1) return 1;
+    for (int t = 0; t < 3; ++t) {
+      const int64_t bk = block_k(t);
+      if (!strcmp(op, "forward")) {
+        printf("hit %s\n", forward(t, 0, true, a[0], a[1], a[2]).c_str());
+        for (int i = 0; i < 3; ++i) printf("hit %s\n", forward(t, i, false, a[0], a[1], a[2]).c_str());
+      } else if (!strcmp(op, "dx")) {
+        for (int two = 0; two < 2; ++two)
+          for (int e = 0; e < 2; ++e) printf("hit %s\n", dx(t, e, a[0], a[2], ceil_div(a[1], bk) + two * ceil_div(a[1] + 5, bk)).c_str());
+      } else if (!strcmp(op, "dw")) {
+        dpvo_gated_linear_dw_t p = {};
+        p.M = a[0], p.n = (n - 1) / 2, p.dtype = t;
+        for (int i = 0; i < p.n; ++i) p.N[i] = a[1 + 2 * i], p.K[i] = a[2 + 2 * i];
+        printf("hit %s\n", key(F_TN, E_LIN, t, dw_plan(&p)).c_str());
+      } else {                                            // norm: rows, D, gate rows (0: no gate), a branch (1: behind a norm with parameters)
+        dpvo_residual_norm_t p = {};
+        char x;
+        p.M = a[0], p.D = (int)a[1], p.groups = a[2], p.gate = a[2] ? &x : nullptr, p.f = a[3] ? &x : nullptr, p.x_dtype = t, p.dw = p.db = &x;
+        if (a[3]) p.dgate = p.gate ? &x : nullptr;
+        if (a[3] == 1) p.dpw = p.dpb = &x;
+        const NormPlan c = norm_plan(p);
+        const int fs = norm_shape(p, false, 0);
+        printf("norm %d %d %ld %ld %ld %ld %ld %ld %d %d %ld\n", t, c.sh, (long)c.groups, (long)c.rpg, (long)c.gpb, (long)c.bpg, (long)c.blocks, (long)norm_slots(c.sh), c.shared, fs,
+               (long)norm_slots(fs));
+      }
+    }
+  }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def paths(tmp_path_factory):
+    """the library's rules, by themselves: what they return over a grid of sizes, and for the sizes that the GPU tests list"""
+    from tests import test_gpu_blocks_paths as G
+    d = tmp_path_factory.mktemp("paths")
+    (d / "paths.cpp").write_text(PATHS)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "dpvo_amd", "csrc"), "-I", os.path.join(ROOT, "include"), str(d / "paths.cpp"), "-o", str(d / "paths")])
+    cases = [("forward", *c) for c in G.FORWARD] + [("dx", *c) for c in G.INPUT_GRADIENTS] + [("dw", M, *(n for s in sizes for n in s)) for M, sizes in G.WEIGHT_GRADIENTS]
+    for lead, D, gate in G.NORMS + G.NORMS_PLAIN:
+        rows, groups = 1, 1
+        for n in lead:
+            rows *= n
+        for n in gate or (0,):
+            groups *= n
+        cases.append(("norm", rows, D, groups, 1 if (lead, D, gate) in G.NORMS else 2))
+    cases += [("norm", M, D, 0, 0) for M, D in G.NORM_ALONE]
+    text = "\n".join(" ".join(map(str, (c[0], len(c) - 1, *c[1:]))) for c in cases)
+    out = subprocess.run([str(d / "paths")], input=text, capture_output=True, text=True, check=True).stdout.splitlines()
+    kept = {k: [l[len(k) + 1:] for l in out if l.startswith(k + " ")] for k in ("all", "hit", "norm")}
+    assert sum(map(len, kept.values())) == len(out)
+    return kept
+
+
+def test_the_gpu_tests_reach_every_product(paths):
+    every, reached = set(paths["all"]), set(paths["hit"])
+    assert len(every) > 60 and not every - reached, sorted(every - reached)
+    assert not reached - every, sorted(reached - every)                          # (the grid is wide enough)
+
+
+def test_no_product_is_built_that_nothing_reaches(paths):
+    """the tile kernels in the library, by form, epilogue and tile, as many of each as there are types that choose it"""
+    import collections
+    import re
+    import shutil
+    if not shutil.which("nm"):
+        pytest.skip("no nm")
+    names = {"nt": 0, "nn": 1, "tn": 2}, {"lin": 0, "gate": 1, "gate2": 2, "dact": 3}, {"tile": 0, "big": 1, "small": 2, "tiny": 3}
+    want = collections.Counter()
+    for k in {tuple(k.split()[:4]) for k in paths["all"]}:
+        if k[3] in names[2]:
+            want[tuple(n[x] for n, x in zip(names, k[1:]))] += 1 if k[0] == "f32" else 2
+    out = subprocess.check_output(["nm", "-C", L.LIB_PATH], text=True)
+    have = collections.Counter(tuple(map(int, m)) for m in re.findall(r" [dD] void blk::\(anonymous namespace\)::gemm_kernel<(\d), (\d), (\d)>\(", out))
+    assert have == want
+
+
+def test_the_gpu_tests_reach_the_loops_of_the_norms(paths):
+    """backward: for every number of lanes a workgroup with several rounds of rows, with several groups, and the last of them short; with parts of a
+    group of several rounds; forward: workgroups that go round.  (Shapes: blocks_plan.h's NORM_SHAPES, 12 the 1024 lanes, 13 the wide rows)"""
+    rounds, groups, short, parts, forward = set(), set(), set(), set(), set()
+    for l in paths["norm"]:
+        t, sh, n, rpg, gpb, bpg, blocks_, slots, shared, fsh, fslots = map(int, l.split())
+        if -(-rpg // slots) >= 2 * bpg:
+            rounds.add(sh)
+        if gpb > 1:
+            groups.add(sh)
+            if n % gpb:
+                short.add(sh)
+        if shared and bpg > 1 and -(-rpg // slots) >= 2 * bpg:
+            parts.add(sh)
+        rows, D = n * rpg, None
+        most = {13: 8192}.get(fsh, 2048 if 6 <= fsh <= 11 else 8192)
+        if rows > most * fslots:
+            forward.add(fsh)
+    every = set(range(14))
+    assert rounds == every, every - rounds
+    assert forward == every - {12}, every - forward                              # (the 1024 lanes go backward only)
+    assert groups == every, every - groups
+    assert len(short) >= 8 and 13 in short and 12 in short, short
+    assert len(parts) >= 8 and {2, 8, 12, 13} <= parts, parts
