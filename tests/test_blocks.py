@@ -594,3 +594,23 @@ def test_the_gpu_tests_reach_the_loops_of_the_norms(paths):
     assert groups == every, every - groups
     assert len(short) >= 8 and 13 in short and 12 in short, short
     assert len(parts) >= 8 and {2, 8, 12, 13} <= parts, parts
+
+
+def test_the_gpu_tests_bounds_see_a_mistake():
+    """the oracle with mistakes planted, on the host: bounds, exact products, sums over rows"""
+    from tests import test_gpu_blocks as B, test_gpu_blocks_paths as G
+    B.test_the_bounds_see_a_mistake()
+    g = torch.Generator().manual_seed(0)
+    a, b = (torch.randint(-1, 2, (3000, n), generator=g).double() for n in (40, 30))
+    right = a.t() @ b
+    for t in (torch.float16, torch.bfloat16, torch.float32):
+        G.exactly(right.to(t), right, t, "right")
+        for rows in (slice(0, 2999), slice(64, 3000), slice(0, 2936)):           # one row, a first or a last block of the sum left out
+            with pytest.raises(AssertionError):
+                G.exactly((a[rows].t() @ b[rows]).to(t), right, t, "planted")
+    q = B.V(torch.randn(3000, 20, generator=g, dtype=torch.float64) + 0.5)
+    want = G.sum_rows(q, 3000)
+    B.within(q.v.float().sum(0, keepdim=True), want, torch.float32, "right")
+    for wrong in (q.v[:2999], q.v[64:], q.v[::2] * 2):
+        with pytest.raises(AssertionError):
+            B.within(wrong.float().sum(0, keepdim=True), want, torch.float32, "planted")

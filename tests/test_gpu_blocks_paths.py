@@ -222,3 +222,33 @@ def test_norm_alone_rows(dev, tx, th, M, D):
     within(dx, norm_back(R(dh) * R(w), xh, r, kind), tx, "dx")
     within(dw, sum_rows(R(dh) * xh, M), tx, "dw")
     within(db, sum_rows(R(dh), M), tx, "db")
+
+
+@pytest.mark.parametrize("tb", [F16, BF16], ids=str)
+@pytest.mark.parametrize("lead,D,gate", [((5,), 7, (5,)), ((300,), 384, (1,)), ((40, 3), 385, (40, 1)), ((9,), 2056, None), ((30,), 3001, (30,)), ((20,), 4104, (1,)), ((11,), 9001, (11,))])
+def test_f32_rows_behind_a_16_bit_branch(dev, tb, lead, D, gate):
+    """x, s and h in f32, branch and gate in 16 bits (`out_dtype` x's): h's gradient arrives in f32"""
+    g = gen(D, *lead, 5)
+    r = lambda *s, t, mean=0.0: (torch.randn(*s, generator=g, device=dev) + mean).to(t).requires_grad_()  # noqa: E731
+    x, f, w, b = r(*lead, D, t=F32), r(*lead, D, t=tb), r(D, t=F32, mean=1.0), r(D, t=F32)
+    ga = None if gate is None else r(*gate, D, t=tb)
+    ds, dh = r(*lead, D, t=F32).detach(), r(*lead, D, t=F32).detach()
+    s, h = blocks.residual_norm(x, f, w, b, gate=ga, gate_activation="silu", out_dtype=F32)
+    M = x.numel() // D
+    R = lambda q: V(q.detach().double().reshape(-1, D))  # noqa: E731
+    par = lambda q: V(q.detach().double())  # noqa: E731
+    A, dA = (V(torch.ones(M, D, dtype=torch.float64, device=dev)), None) if ga is None else act("silu", V(ga.detach().double().expand(*lead, D).reshape(M, D)))
+    S = R(x) + R(f) * A
+    within(s, S, F32, "s")
+    sh, sr = normalise(S, "layer", 1e-3)
+    within(h, sh * par(w) + par(b), F32, "h")
+    leaves = {"x": x, "f": f, "w": w, "b": b, **({} if ga is None else {"gate": ga})}
+    grads = dict(zip(leaves, torch.autograd.grad([s, h], list(leaves.values()), [ds, dh])))
+    DY = norm_back(R(dh) * par(w), sh, sr, "layer") + R(ds)
+    within(grads["x"], DY, F32, "dx")
+    within(grads["f"], DY * A, tb, "df")
+    within(grads["w"], sum_rows(R(dh) * sh, M), F32, "dw")
+    within(grads["b"], sum_rows(R(dh), M), F32, "db")
+    if ga is not None:
+        dga, k = DY * R(f) * dA, M // (ga.numel() // D)
+        within(grads["gate"], dga if k == 1 else sum_rows(dga, k), tb, "dgate")
