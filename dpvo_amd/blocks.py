@@ -43,28 +43,45 @@ def _code(table, key, what, arg):
         _fail(what, f"{arg} is {key!r}, not one of {', '.join(map(repr, table))}")
 
 
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _modes, _PROXY = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._TorchDispatchModeKey.PROXY
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 
 
-def _check_plain(what, *tensors):
-    """the kernels read and write memory behind torch's back: refuses what would get lost there"""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _fail(what, "forward-mode derivatives are not provided, and an input is a dual tensor")
-    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
+def _check_recording(what, tensors):
+    """the kernels read and write memory behind torch's back: what would record a call sees nothing of it"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _fail(what, "forward-mode derivatives are not provided, and an input is a dual tensor")
+    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None):
         _fail(what, "a call under torch.jit.trace or make_fx: what the kernels write is not recorded, a trace would return memory as it was")
+
+
+def _check_type(what, t):
+    if type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+        _fail(what, f"a {type(t).__name__}, whose values do not lie in memory of its own")
+
+
+def _check_gradients(what, *tensors):
+    """those that arrive"""
+    if forward_ad._current_level >= 0 or _is_tracing() or _modes():
+        _check_recording(what, tensors)
     for t in tensors:
-        if type(t) is not torch.Tensor and t is not None and type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
-            _fail(what, f"a {type(t).__name__}, whose values do not lie in memory of its own")
+        if type(t) not in _PLAIN:
+            _check_type(what, t)
 
 
 def _check(what, x, *others):
-    """one device, a dtype that the kernels know"""
-    _check_plain(what, x, *others)
+    """tensors whose values lie in their memory, a call that nothing else records, one device, a dtype that the kernels know"""
+    if forward_ad._current_level >= 0 or _is_tracing() or _modes():
+        _check_recording(what, (x, *others))
+    if type(x) not in _PLAIN:
+        _check_type(what, x)
+    i = x.get_device()
     for t in others:
-        if t is not None and t.device != x.device:
-            _fail(what, f"tensors on {x.device} and {t.device}")
+        if t is not None:
+            if type(t) not in _PLAIN:
+                _check_type(what, t)
+            if t.get_device() != i or (i < 0 and t.device != x.device):
+                _fail(what, f"tensors on {x.device} and {t.device}")
     if x.dtype not in _DTYPES:
         _fail(what, f"unsupported dtype {x.dtype} (float16, bfloat16, float32)")
 
@@ -276,7 +293,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _check_plain("linear", dy)
+        _check_gradients("linear", dy)
         x, w, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         with _on(x):
@@ -314,7 +331,7 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _check_plain("gated_linear", dy)
+        _check_gradients("gated_linear", dy)
         x, v, wg, wu, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dv = dwg = dwu = dbg = dbu = None
@@ -369,7 +386,7 @@ class _FeedForward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _check_plain("gated_feed_forward", dy)
+        _check_gradients("gated_feed_forward", dy)
         x, wg, wu, wd, h, g, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dwu = dbg = dbu = None
@@ -424,7 +441,7 @@ class _GatedResidual(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        _check_plain("gated_residual", dy)
+        _check_gradients("gated_residual", dy)
         x, wg, w1, w2, t, g, r = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dwg = dbg = dw1 = db1 = dw2 = db2 = None
@@ -524,7 +541,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, ds, dh):
-        _check_plain("residual_norm", ds, dh)
+        _check_gradients("residual_norm", ds, dh)
         x, f, gate, w, b, pw, pb = ctx.saved_tensors
         grads = [None] * 7
         if ds is None and dh is None:
