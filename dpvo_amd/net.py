@@ -21,6 +21,7 @@ from .graph import GraphPlan
 from .utils import coords_grid_with_index
 
 DIM = 384
+_raw_stream = blocks._raw_stream
 
 # bench.py sets this to a list to collect (start_event, end_event, n_edges) of every Update.forward: HIP events recorded on the
 # launch stream around the operator (MFMA roofline measurement); None = no overhead.
@@ -245,18 +246,31 @@ class Update(nn.Module):
         """f16 weight images for the kernels.  Loading, moving and casting parameters, and training `gru`, are followed by themselves (operands());
         re-run it after any other change of them."""
         for m in self._stages():
-            del m.__dict__["stale"]
+            m.__dict__.pop("stale", None)
         return self._pack()
 
     def operands(self):
-        """the images for a call: those at hand, or new ones where the parameters have changed, or may have (a stage that is being trained)"""
+        """the images for a call: those at hand, or new ones where the parameters have changed, or may have (a stage that is being trained).  On a
+        stream that has not used them yet: behind the launches that write them, and their memory is kept for what the stream has under way"""
         stages = self._stages()
-        if self._packed is not None and not stages:
-            return self._packed
-        for m in stages:
-            if m.stale < 2:
-                del m.__dict__["stale"]
-        return self._pack()
+        P = self._packed
+        if P is None or stages:
+            for m in stages:
+                if m.stale < 2:
+                    m.__dict__.pop("stale", None)
+            P = self._pack()
+        seen = P.get("_streams")
+        if seen is not None:
+            dev = P["norm"][0].get_device()
+            stream = _raw_stream(dev)
+            if stream not in seen and not torch.cuda.is_current_stream_capturing():      # (a capture starts with a synchronisation)
+                cur = torch.cuda.current_stream(dev)
+                cur.wait_event(P["_written"])
+                for v in P.values():
+                    for t in v if isinstance(v, (tuple, list)) else ():
+                        t.record_stream(cur)
+                seen.add(stream)
+        return P
 
     def _pack(self):
         h = lambda t: t.detach().to(torch.float16).contiguous()
@@ -309,6 +323,8 @@ class Update(nn.Module):
             fp.d_w, fp.d_b, fp.w_w, fp.w_b = (t.data_ptr() for t in (*P["d"], *P["w"]))
             fp.tiling, fp.start_skew = self.tiling, self.start_skew
             P["_fparams"] = fp
+            if not torch.cuda.is_current_stream_capturing():
+                P["_written"], P["_streams"] = torch.cuda.current_stream(dev).record_event(), {_raw_stream(dev.index)}
         self._packed = P
         return P
 

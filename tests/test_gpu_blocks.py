@@ -998,3 +998,37 @@ def test_gates_of_a_f32_stream_are_f32(dev, tb, a, D):
     s, _ = blocks.residual_norm(x, one, norm=None, gate=gate, gate_activation=a, post_norm="rms", post_weight=pw, post_bias=pb)
     got, = torch.autograd.grad(s, pb, torch.ones_like(s))
     within(got, V(v, 5 * U * v.abs()), F32, "d post_bias")
+
+
+def test_operand_images_on_another_stream(dev):
+    """images that one stream has yet to write are used by a call on another only behind that, and last until that call is done"""
+    from dpvo_amd import net as N
+    from tests import helpers as H
+    torch.manual_seed(7)
+    upd = N.Update(3).to(dev)
+    ii, jj, kk, _ = H.small_graph(14, 8)
+    E = ii.numel()
+    ii, jj, kk = ii.to(dev), jj.to(dev), kk.to(dev)
+    g = torch.Generator().manual_seed(0)
+    net, inp, corr = (torch.randn(1, E, n, generator=g).cuda() * s for n, s in ((384, 1.0), (384, 0.5), (882, 0.5)))
+    call = lambda: upd(net, inp.half(), corr.half(), None, ii, jj, kk)[0]  # noqa: E731
+    want = call()
+    busy = torch.randn(8192, 8192, device=dev)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        assert torch.equal(call(), want)                                        # (plan and workspaces of this stream)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        y = busy
+        for _ in range(6):
+            y = y @ busy * 1e-4                                                 # some tens of milliseconds in front of the images
+        upd.pack()
+        kept = [torch.full_like(t, float("nan")) for t in upd._packed["_fw"]]   # (behind them: over memory that the last images left)
+        with torch.cuda.stream(other):
+            got = call()
+            upd.pack()                                                          # the images of the call are dropped while it runs
+            more = [torch.full_like(t, float("nan")) for t in upd._packed["_fw"]]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del kept, more
