@@ -361,8 +361,9 @@ extern "C" int dpvo_residual_norm(const dpvo_residual_norm_t* p, void* stream) {
   a.p = *p;
   a.rows_per_gate = p->gate ? (uint32_t)(p->M / p->groups) : 1;
   const int sh = norm_shape(*p, false, 0);
-  // (ragged rows profit from several to a workgroup, whose loads then run ahead: 4096 x 2333 bf16 49 against 57 us, 8192 x 1001 24 against 32; of
-  //  whole pieces 8192 x 4096 takes 73 us with a workgroup to a row, 79 with 2048 workgroups)
+  // Ragged rows profit from several to a workgroup, whose loads then run ahead: `norm` of 4096 x 2333 bf16 27 us with 2048 workgroups, 35 with 8192,
+  // 45312 x 385 27 and 42, f32 29 and 39.  Rows of whole pieces: with two inputs in f32 8192 loses nothing and 2048 up to 8 % (45312 x 384 51 and 55 us,
+  // 16384 x 4000 194 and 201); in 16 bits 2048 would be faster, by 8 to 24 % for `norm` alone (8192 x 4096 38 and 31 us) and 0 to 10 % with a branch.
   const int64_t want = cdiv64(p->M, norm_slots(sh)), most = p->D % 8 ? 2048 : 8192;
   return norm_run(a, sh, false, want < most ? want : most, (hipStream_t)stream);
 }

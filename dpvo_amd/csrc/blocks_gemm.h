@@ -368,6 +368,9 @@ template <int FORM, int EPI, int KIND> __global__ void __launch_bounds__(Cfg<KIN
     }
   }
 
+  // Roundings: everything here is f32 up to the stores.  What is stored in T is what the matrix unit takes in T: a hidden product or layer (E_GATE,
+  // E_LIN with an activation) as the next product's operand, dG and dU (E_DACT) as those of dx and dw; a bias's gradient sums the same rounded values,
+  // so that it is the gradient of the operand that was used.  A second, finer operand would double the products.
   // ---- epilogue: 32 rows at a time through the wave's own piece of LDS (the last barrier of the loop freed it), then along rows.  Where there
   // are two sums, or an activation, a rolled loop does the work (the activations are long); where there is one, what follows it is short and
   // unrolled, and what that needs from memory (a residual, a mask) is requested for all its rows beforehand, so that a piece waits once

@@ -9,11 +9,13 @@
 //   dy = ds + J_norm(s)^T dh;  dx = dy;  q = scale * dy;  dgate = q * p * act'(gate);  dp = q * act(gate);  df = J_post(f)^T dp
 //   J^T d = r (d w - mean(d w) - xhat mean(d w xhat))   (rms: without the first mean), with xhat the normalised row and r its factor
 //
-// A row lives in the registers of L lanes, so every tensor is read once and statistics are two-pass in f32 at no traffic; the next row's loads
-// are under way while a row is computed.  Nothing but memory bounds these kernels.  Gradients of what all rows (of a group) share are summed
-// in LDS over a workgroup's rows, then over its row slots, then over workgroups by a second launch: no atomics, the order is fixed.
-// Measured: 45312 x 384 with f32 stream, f16 branch and gate forward 44 us (5.6 TB/s; a large copy reaches 5.0 to 6.8); 8192 x 4096 bf16 with both
-// norms and a gate for each of four groups forward 54 us (5.0 TB/s), backward 115 + 6 us (3.5 TB/s: the sums in LDS and spilled registers, below).
+// Rows of up to 4096 elements: a row lives in the registers of L lanes, so every tensor is read once and statistics are two-pass in f32 at no traffic;
+// the next row's loads are under way while a row is computed.  Nothing but memory bounds the forward kernels.  Gradients of what all rows (of a group)
+// share are summed in LDS over a workgroup's rows, then over its row slots, then over workgroups by a second launch: no atomics, the order is
+// fixed; the sums in LDS and spilled registers bound the backward.  Wider rows: what does
+// not fit the registers is read again from L2, and backward the sums over rows are a second kernel, which reads the inputs again (below).
+// Measured: 45312 x 384 with f32 stream, f16 branch and gate forward 46 us (5.3 TB/s; a large copy reaches 5.0 to 6.8); 8192 x 4096 bf16 with both
+// norms and a gate for each of four groups forward 54 us (5.0 TB/s), backward 115 + 6 us (3.5 TB/s).
 #pragma once
 #include "blocks_dev.h"
 
@@ -332,7 +334,9 @@ template <class NX, class NB, int L, bool RAGGED> __global__ void __launch_bound
   apw.init(p.dpw, room);
   apb.init(p.dpb, room);
   ag.init(a.part_gate, room);
-  constexpr bool KEEP = L < 1024;                        // the weights stay in registers where there is room
+  // The weights stay in registers up to 512 lanes: 8192 x 4096 bf16 104 us, read again for each row 117; 45312 x 384 64 and 72, f32 97 and 119; narrow
+  // rows of 16 bits lose (131072 x 128: 92 and 59), and 1024 lanes would gain (4096 x 8192 bf16 121 us kept, 131 read again).
+  constexpr bool KEEP = L < 1024;
   float kw[P], kpw[P];
   if constexpr (KEEP) {
     row.param(p.w, p.w_dtype, 1.f, kw);
@@ -713,9 +717,8 @@ template <class NX, class NB> __global__ void __launch_bounds__(256, 2) norm_col
   if (p.dpb) row.put(a.part_pb + o, 0, apb);
 }
 
-// (512 threads with 16 elements each where those are enough: two workgroups on a compute unit take turns at their barriers.  4096 x 8192 bf16, forward and
-// first backward kernel: 87 and 145 us, 101 and 215 with 1024 threads of 8; 2048 x 16384: 92 and 170 with 1024 of 16, 121 and 199 with 512 of 32.
-// Since whole pieces have kernels of their own: 75 and 126, 73 and 143)
+// (512 threads with 16 elements each where those are enough, as two workgroups on a compute unit take turns at their barriers; 1024 with 16 for wider
+// rows.  Whole pieces, bf16, forward and first backward kernel: 4096 x 8192 75 and 126 us, 2048 x 16384 73 and 143)
 template <class NX, class NB, int L, bool RAGGED> int norm_wide(const NormArgs& a, bool back, int64_t blocks, hipStream_t s) {
   const dim3 rows((unsigned)(a.p.M < 8192 ? a.p.M : 8192));
   if (!back) hipLaunchKernelGGL((norm_wide_kernel<NX, NB, L, 2, RAGGED>), rows, dim3(L), 0, s, a);

@@ -73,6 +73,9 @@ inline Plan linear_plan(const dpvo_gated_linear_t* p, int epi) {
 //  - for 16-bit rows of odd length, whose unaligned pieces the tiles load once and these workgroups again and again (96 x 882 x 385: 14.9 against
 //    9.0 us, with 386 columns 7.7 against 8.1; by the length and not the address, so that a result does not depend on where its operands lie),
 //  - for long sums that may be cut into parts (f16 96 x 1024 x 4096: 20.1 against 14.8 us, 96 x 768 x 2048 11.5 against 11.8).
+// Sums of any length that cannot be cut (a gate, an activation) stay here: M x K x N, one input / two inputs / one product with an activation, against
+// tiles, in us: f16 48 x 4096 x 4096 24 / 33 / 18 against 43 / 78 / 41, 96 x 8192 x 1024 45 / 72 / 37 against 80 / 150 / 51, 1000 x 8192 x 256
+// 46 / 73 / 38 against 79 / 144 / 75, 1000 x 2048 x 256 15 / 21 / 12 against 17 / 42 / 16; f32 96 x 8192 x 1024 109 / 152 / 74 against 182 / 380 / 178.
 inline bool linear_few(const dpvo_gated_linear_t* p, int epi) {
   if (p->M <= 16) return true;
   if (ceil_div(p->N, 16) * ceil_div(p->M, 64) > (p->M <= 32 || (epi == E_GATE2 && p->dtype == DPVO_F32) ? 512 : 256)) return false;
