@@ -93,6 +93,9 @@ def _check_layer(what, x, K, w, b, name):
         _fail(what, f"{name} is {tuple(w.shape)}: no features")
     if w.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
         _fail(what, f"{name} and its bias must have the input's dtype {x.dtype}")
+    most = _MAX_LD[x.element_size()]
+    if K > most or (w.shape[0] > most and _wants_grad(x, w, b)):           # (forward alone, outputs are addressed with 64 bits)
+        _fail(what, f"{name} is {tuple(w.shape)}: rows of at most {most} elements, and in the backward pass outputs too")
     if b is not None and tuple(b.shape) != (w.shape[0],):
         _fail(what, f"the bias of {name} is {tuple(b.shape)}, not ({w.shape[0]},)")
 

@@ -614,3 +614,28 @@ def test_the_gpu_tests_bounds_see_a_mistake():
     for wrong in (q.v[:2999], q.v[64:], q.v[::2] * 2):
         with pytest.raises(AssertionError):
             B.within(wrong.float().sum(0, keepdim=True), want, torch.float32, "planted")
+
+
+@pytest.mark.parametrize("t,most", [(H, 4194303), (torch.bfloat16, 4194303), (torch.float32, 2097151)], ids=str)
+def test_rows_that_are_too_long_are_refused_before_any_launch(t, most):
+    e = lambda *s: torch.empty(*s, dtype=t)  # noqa: E731
+    long, too = e(1, most), e(1, most + 1)
+    with pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+        blocks.linear(long, long)
+    with pytest.raises(L.DPVOHipError, match="rows of at most"):
+        blocks.linear(too, too)
+    with pytest.raises(L.DPVOHipError, match="rows of at most"):
+        blocks.gated_linear(e(1, 4), e(1, 4), too, up_input=too)
+    with pytest.raises(L.DPVOHipError, match="rows of at most"):
+        blocks.gated_feed_forward(e(1, 4), e(most + 1, 4), e(most + 1, 4), e(2, most + 1))
+    # as many outputs: a gradient's rows, so only where one will be asked for
+    x, w = e(1, 2), e(most + 1, 2)
+    with pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+        blocks.linear(x, w)
+    for leaf in (x, w):
+        leaf.requires_grad_()
+        with pytest.raises(L.DPVOHipError, match="rows of at most"):
+            blocks.linear(x, w)
+        with torch.no_grad(), pytest.raises(L.DPVOHipError, match="run on the GPU only"):
+            blocks.linear(x, w)
+        leaf.requires_grad_(False)
