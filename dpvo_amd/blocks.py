@@ -13,8 +13,9 @@ products run on the matrix cores, sums, statistics and activations are float32. 
 type, as the matrix cores take it: the hidden product act(..) * (..), and in the backward pass the gradients of the sums (which the activations'
 derivatives read in float32, as saved).  So a 16-bit block's results are a step or two of its type's rounding away from the formula's, and its
 gradients need the loss scaled as those of any 16-bit operands.  Everything runs on the current stream of the tensors' device.
-Gradients of first order are provided, in reverse mode (dual tensors are refused); results and gradients do not vary from run to run.  Autocast is not consulted.  A backward pass that is
-captured into a graph follows PyTorch's rule: no eager graph of the same leaves may be alive."""
+Gradients of first order are provided, in reverse mode; results and gradients do not vary from run to run.  Autocast is not consulted.  Dual tensors,
+torch.jit.trace, make_fx and tensors without memory of their own are refused.  A backward pass that is captured into a graph follows PyTorch's rule:
+no eager graph of the same leaves may be alive."""
 import ctypes
 
 import torch
