@@ -332,6 +332,9 @@ class Update(nn.Module):
         self._packed = None
         return super()._apply(fn, *a, **k)
 
+    def __getstate__(self):                              # (copies and pickles make images of their own: these hold device addresses)
+        return {**self.__dict__, "_packed": None}
+
     def _load_from_state_dict(self, *a, **k):            # (of a whole network's load too)
         self._packed = None
         return super()._load_from_state_dict(*a, **k)

@@ -639,3 +639,21 @@ def test_rows_that_are_too_long_are_refused_before_any_launch(t, most):
         with torch.no_grad(), pytest.raises(L.DPVOHipError, match="run on the GPU only"):
             blocks.linear(x, w)
         leaf.requires_grad_(False)
+
+
+def test_a_packed_network_can_be_copied():
+    """an average of the weights, or a checkpoint of the whole module, taken while the tracker's images are there"""
+    import copy
+    import io
+    from dpvo_amd import net as N
+    network = N.VONet()
+    P = network.update.pack()
+    twin = copy.deepcopy(network)
+    buf = io.BytesIO()
+    torch.save(network, buf)
+    assert network.update.operands() is P
+    with torch.no_grad():
+        twin.update.gru[1].res[2].weight.add_(1)
+    a, b = P["g0"][4], twin.update.operands()["g0"][4]
+    assert torch.equal(b, twin.update.gru[1].res[2].weight.half()) and not torch.equal(a, b) and network.update.operands() is P
+    assert all(torch.equal(p, q) for p, q in zip(twin.state_dict().values(), network.state_dict().values()) if p.shape != (384, 384))
